@@ -51,7 +51,10 @@ typedef enum dwbnq_status {
   DWBNQ_ERR_DEVICE_FLAG = 6  /* a kernel recorded an internal error (bounded wait)    */
 } dwbnq_status;
 
-typedef enum dwbnq_dtype { DWBNQ_F32 = 0, DWBNQ_F16 = 1 } dwbnq_dtype;
+/* DWBNQ_BF16 (bfloat16 in memory, fp32 arithmetic, one rounding at the store) is taken by the
+ * entry points of the affine layer in few bits only (from dwbnq_ckpt8_store on); the others
+ * refuse it. */
+typedef enum dwbnq_dtype { DWBNQ_F32 = 0, DWBNQ_F16 = 1, DWBNQ_BF16 = 2 } dwbnq_dtype;
 
 typedef enum dwbnq_quant_kind {
   DWBNQ_Q_NONE = 0,  /* conv (+BN) only                                   */
@@ -316,7 +319,13 @@ typedef enum dwbnq_pw_math { DWBNQ_PW_MATH_FP32 = 0, DWBNQ_PW_MATH_TF32 = 1 } dw
 /* Activation between BatchNormalization and the quantizer: ReLU is max(0, x)
  * (src/nbla/cuda/function/generic/relu.cu:31-41), ReLU6 is min(max(x, 0), 6)
  * (src/nbla/cuda/function/generic/relu6.cu:25-26). */
-typedef enum dwbnq_act { DWBNQ_ACT_NONE = 0, DWBNQ_ACT_RELU = 1, DWBNQ_ACT_RELU6 = 2 } dwbnq_act;
+typedef enum dwbnq_act {
+  DWBNQ_ACT_NONE = 0,
+  DWBNQ_ACT_RELU = 1,
+  DWBNQ_ACT_RELU6 = 2,
+  DWBNQ_ACT_SILU = 3, /* x / (1 + e^-x); gated unit only            */
+  DWBNQ_ACT_GELU = 4  /* x erfc(-x / sqrt 2) / 2; gated unit only   */
+} dwbnq_act;
 
 /* Geometry of Convolution(ctx, base_axis, pad, stride, dilation, group, channel_last)
  * (include/nbla/cuda/function/convolution.hpp:27-33) restricted to the pointwise case the
@@ -380,6 +389,100 @@ int dwbnq_pwconv_fused_fwd_prepared(const dwbnq_pwconv_desc *desc, const dwbnq_q
  * exact for binary16 factors, whatever `math` says), 0 = the plain FMA kernel (other c_in).
  * Diagnostic only. */
 int dwbnq_pwconv_plan(const dwbnq_pwconv_desc *desc, const void *x, const void *w, int *path_out);
+
+/* ---- the affine layer of a transformer in few bits --------------------------------------- */
+
+/* Training keeps a layer's input from the forward to the backward pass; these entry points keep
+ * it in 8 bits and read it there. Serving reads every weight once per token; these read weights of
+ * 4 bits. The affine layer is Affine(x, w, b) of the reference (include/nbla/cuda/function/
+ * affine.hpp) for row vectors - what Convolution 1x1 is at h = w = 1 - with the weight stored
+ * [c_out, c_in] as there.
+ *
+ * 8-bit checkpoint of a tensor [rows, cols]: every row is cut into groups of 32 consecutive
+ * values (the last group of a row may be short). A group has one byte b = max(7, biased fp32
+ * exponent of its largest magnitude), which gives the step delta = 2^(b - 133), and each value
+ * x one int8 code k = clamp(round_half_even(x / delta), -127, 127); it stands for k * delta.
+ * |x - k delta| <= delta / 2 up to 127.5 delta and < delta above; largest magnitude / delta lies in
+ * [64, 128) (lower for magnitudes below 2^-120, where the step stays 2^-126). A group that holds
+ * a NaN or an infinity has b = 255 and codes 0 and stands for NaN throughout. The arithmetic is
+ * exact, so the result is the same bit for bit whoever computes it.
+ *   codes: int8 [rows, 32 * ceil(cols / 32)], 16-byte aligned; codes past cols are written as 0
+ *          (and what stands there is ignored by no reader: keep them 0);
+ *   exps:  uint8 [rows, ceil(cols / 32)].
+ * Row strides (ld_*) count elements, are at least cols, and may take any value and alignment;
+ * strides that are multiples of 16 bytes on 16-byte aligned tensors are faster. rows, cols (c_in,
+ * c_out) may be 0: then nothing is read, and gradients are those of an empty batch. */
+int dwbnq_ckpt8_store(int dtype, int64_t rows, int64_t cols, int64_t ld_x, const void *x, void *codes,
+                      void *exps, int device, void *stream);
+/* y = the values the checkpoint stands for, rounded to dtype (exact for DWBNQ_F32 and DWBNQ_BF16). */
+int dwbnq_ckpt8_load(int dtype, int64_t rows, int64_t cols, const void *codes, const void *exps, int64_t ld_y,
+                     void *y, int device, void *stream);
+
+/* Gated unit of a transformer MLP: y = act(gate) * up, act one of DWBNQ_ACT_SILU, _GELU, _RELU,
+ * fp32 arithmetic rounded once. gate_codes .. up_exps: all four given, the checkpoints of gate
+ * and up are written in the same pass; all four NULL, the bare forward. gate and up are
+ * typically the two halves of one projection's output. y may be gate or up itself (same
+ * address and stride); other overlaps are not allowed. */
+int dwbnq_glu_fwd(int dtype, int act, int64_t rows, int64_t cols, int64_t ld_gate, const void *gate, int64_t ld_up,
+                  const void *up, int64_t ld_y, void *y, void *gate_codes, void *gate_exps, void *up_codes,
+                  void *up_exps, int device, void *stream);
+/* Its backward from the two checkpoints: dgate (+)= dy * up * act'(gate), dup (+)= dy * act(gate), with
+ * the values the checkpoints stand for. dgate and dup may each be NULL (propagate_down false; dy
+ * is then only needed for the other). prod_codes and prod_exps (both or neither) receive the
+ * checkpoint of act(gate) * up, the input of the layer behind the unit, so that layer needs
+ * none of its own. accum_mask bit 0 / 1: accumulate onto dgate / dup. dgate or dup may be dy
+ * itself (same address and stride). */
+int dwbnq_glu_bwd_ckpt8(int dtype, int act, int64_t rows, int64_t cols, const void *gate_codes, const void *gate_exps,
+                        const void *up_codes, const void *up_exps, int64_t ld_dy, const void *dy, int64_t ld_dgate,
+                        void *dgate, int64_t ld_dup, void *dup, void *prod_codes, void *prod_exps, int accum_mask,
+                        int device, void *stream);
+
+/* Geometry of the affine layer's backward. */
+typedef struct dwbnq_affine_desc {
+  int32_t dtype;    /* of dy                                                       */
+  int32_t dw_dtype; /* of dw and db: dtype, or DWBNQ_F32 (gradients kept in 32 bits) */
+  int64_t rows;     /* tokens                                                      */
+  int32_t c_in, c_out;
+  int64_t ld_dy;    /* row stride of dy, >= c_out                                  */
+} dwbnq_affine_desc;
+/* Bytes of device scratch dwbnq_affine_bwd_ckpt8 needs, 256-byte aligned, contents irrelevant on
+ * entry; calls that may overlap on the GPU need one each. 0 for an invalid descriptor. */
+size_t dwbnq_affine_bwd_workspace_bytes(const dwbnq_affine_desc *desc);
+/* Weight and bias gradients with the input read from its checkpoint (codes and exps of x [rows,
+ * c_in]): dw[o][i] (+)= sum over rows of dy[r][o] * x[r][i], dw [c_out, c_in] contiguous;
+ * db[o] (+)= sum over rows of dy[r][o]. dw and db may each be NULL. accum_mask bit 1 / 2:
+ * accumulate onto dw / db (as in dwbnq_dwconv_bwd). Products are exact, sums are kept in fp32, their
+ * order is fixed: the same call gives the same bits. */
+int dwbnq_affine_bwd_ckpt8(const dwbnq_affine_desc *desc, const void *codes, const void *exps, const void *dy, void *dw,
+                           void *db, int accum_mask, void *workspace, int device, void *stream);
+
+/* 4-bit weights of an affine layer: per output channel, groups of `group` consecutive input
+ * channels (the last may be short) share a scale s and, optionally, an integer zero point z
+ * in 0..15 (8 without); the weight is (q - z) * s with q in 0..15. */
+typedef struct dwbnq_w4_desc {
+  int32_t dtype;       /* of x, y, the bias and the scales */
+  int32_t group;       /* 32, 64 or 128                    */
+  int32_t c_in, c_out;
+  int32_t has_zeros;
+} dwbnq_w4_desc;
+/* Round-to-nearest quantization of w [c_out, c_in] (row stride ld_w): s = largest magnitude of
+ * the group / 7, rounded to dtype; q = clamp(round_half_even(w / s), -8, 7) + 8, no zero points
+ * (a group whose s is 0 has q = 8; one that holds a NaN or an infinity stands for NaN).
+ * codes: uint8 [c_out, c_in], one code per byte; scales: dtype [c_out, ceil(c_in / group)]. */
+int dwbnq_w4_quantize(int dtype, int32_t c_out, int32_t c_in, int32_t group, int64_t ld_w, const void *w, void *codes,
+                      void *scales, int device, void *stream);
+/* Lays codes (as above; the upper four bits of each byte are ignored), scales and zero points
+ * (uint8 [c_out, ceil(c_in / group)], NULL without) out for dwbnq_w4_affine_fwd, once per layer.
+ * packed: dwbnq_w4_packed_bytes(desc) bytes, 256-byte aligned. The size is 0 for an invalid
+ * descriptor. */
+size_t dwbnq_w4_packed_bytes(const dwbnq_w4_desc *desc);
+int dwbnq_w4_pack(const dwbnq_w4_desc *desc, const void *codes, const void *scales, const void *zeros, void *packed,
+                  int device, void *stream);
+/* y = x w^T + b for a few rows (one token, or one token of each of a batch of sequences):
+ * x [rows, c_in], y [rows, c_out] with row strides ld_x and ld_y, b [c_out] or NULL. The weights
+ * are read once per 16 rows. Products x * (q - z) are exact and summed in fp32. */
+int dwbnq_w4_affine_fwd(const dwbnq_w4_desc *desc, int64_t rows, int64_t ld_x, const void *x, const void *packed,
+                        const void *b, int64_t ld_y, void *y, int device, void *stream);
 
 /* ---- communicator: the one exchange the path needs (per-channel min/max) ----------- */
 

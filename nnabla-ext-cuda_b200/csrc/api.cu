@@ -74,6 +74,58 @@ int check_dtype(int dtype) {
   return DWBNQ_OK;
 }
 
+// The affine layer in few bits: tensor types, and a matrix of rows x cols with row stride ld.
+int check_dtype_few_bits(int dtype) {
+  if (dtype != DWBNQ_F32 && dtype != DWBNQ_F16 && dtype != DWBNQ_BF16)
+    return fail(DWBNQ_ERR_INVALID_ARG, "dtype %d is none of DWBNQ_F32, DWBNQ_F16 and DWBNQ_BF16", dtype);
+  return DWBNQ_OK;
+}
+constexpr int64_t kMaxSide = (int64_t)1 << 40;  // keeps rows * stride in 64 bits once the product is checked
+int check_matrix(const char *what, int64_t rows, int64_t cols, int64_t ld) {
+  if (rows < 0 || cols < 0 || rows > kMaxSide || cols > kMaxSide)
+    return fail(DWBNQ_ERR_INVALID_ARG, "%s: [%lld, %lld] is not a valid shape", what, (long long)rows, (long long)cols);
+  if (ld < cols) return fail(DWBNQ_ERR_INVALID_ARG, "%s: row stride %lld below %lld columns", what, (long long)ld, (long long)cols);
+  if (rows > 0 && ld > ((int64_t)1 << 60) / rows)
+    return fail(DWBNQ_ERR_INVALID_ARG, "%s: %lld rows of stride %lld exceed the address space", what, (long long)rows, (long long)ld);
+  return DWBNQ_OK;
+}
+int check_ckpt8(const char *what, const void *codes, const void *exps) {
+  if (!codes || !exps) return fail(DWBNQ_ERR_INVALID_ARG, "%s: codes and exps must not be null", what);
+  if (reinterpret_cast<uintptr_t>(codes) % 16) return fail(DWBNQ_ERR_INVALID_ARG, "%s: codes must be 16-byte aligned", what);
+  return DWBNQ_OK;
+}
+// Tensors are read and written element by element somewhere: their address is a multiple of the element size.
+int check_elem(const char *what, const void *p, int dtype) {
+  if (reinterpret_cast<uintptr_t>(p) % (dtype == DWBNQ_F32 ? 4 : 2))
+    return fail(DWBNQ_ERR_INVALID_ARG, "%s is not aligned to its element size", what);
+  return DWBNQ_OK;
+}
+int check_glu_act(int act) {
+  if (act != DWBNQ_ACT_SILU && act != DWBNQ_ACT_GELU && act != DWBNQ_ACT_RELU)
+    return fail(DWBNQ_ERR_INVALID_ARG, "activation %d is none of SILU, GELU and RELU", act);
+  return DWBNQ_OK;
+}
+int check_affine(const dwbnq_affine_desc *d) {
+  if (!d) return fail(DWBNQ_ERR_INVALID_ARG, "affine desc is null");
+  int st = check_dtype_few_bits(d->dtype);
+  if (st != DWBNQ_OK) return st;
+  if (d->dw_dtype != d->dtype && d->dw_dtype != DWBNQ_F32)
+    return fail(DWBNQ_ERR_INVALID_ARG, "dw_dtype %d is neither the type of dy nor DWBNQ_F32", d->dw_dtype);
+  if (d->c_in < 0 || d->c_out < 0 || d->c_in > (1 << 24) || d->c_out > (1 << 24) || d->rows > ((int64_t)1 << 31) - 256)
+    return fail(DWBNQ_ERR_INVALID_ARG, "affine layer [%lld rows] %d -> %d is out of range", (long long)d->rows, d->c_in, d->c_out);
+  return check_matrix("dy", d->rows, d->c_out, d->ld_dy);
+}
+int check_w4(const dwbnq_w4_desc *d) {
+  if (!d) return fail(DWBNQ_ERR_INVALID_ARG, "w4 desc is null");
+  const int st = check_dtype_few_bits(d->dtype);
+  if (st != DWBNQ_OK) return st;
+  if (d->group != 32 && d->group != 64 && d->group != 128)
+    return fail(DWBNQ_ERR_UNSUPPORTED, "group of %d input channels: 32, 64 and 128 are supported", d->group);
+  if (d->c_in < 0 || d->c_out < 0 || d->c_in > (1 << 24) || d->c_out > (1 << 24))
+    return fail(DWBNQ_ERR_INVALID_ARG, "affine layer %d -> %d is out of range", d->c_in, d->c_out);
+  return DWBNQ_OK;
+}
+
 int check_mm(const dwbnq_quant_desc *q, const dwbnq_minmax_ptrs *mm, const void *workspace) {
   if (!mm || !mm->qr_min || !mm->qr_max || !mm->ql_min || !mm->ql_max)
     return fail(DWBNQ_ERR_INVALID_ARG, "MinMaxQuantize needs qr_min, qr_max, ql_min and ql_max");
@@ -655,6 +707,214 @@ int dwbnq_minmaxq_fwd(int dtype, int64_t size0, int32_t channels, int64_t size2,
   st = mm_finish_ranges(dtype, channels, *q, *mm, ws, comm, s);
   if (st != DWBNQ_OK) return st;
   return launch_mm_apply(dtype, size0, channels, size2, x, y, ws, s);
+}
+
+int dwbnq_ckpt8_store(int dtype, int64_t rows, int64_t cols, int64_t ld_x, const void *x, void *codes, void *exps, int device,
+                      void *stream) {
+  clear_error();
+  NvtxRange nvtx_range("dwbnq_ckpt8_store");
+  int st = check_dtype_few_bits(dtype);
+  if (st == DWBNQ_OK) st = check_matrix("x", rows, cols, ld_x);
+  if (st != DWBNQ_OK) return st;
+  if (rows > 0 && cols > 0) {
+    if (!x) return fail(DWBNQ_ERR_INVALID_ARG, "x must not be null");
+    st = check_ckpt8("checkpoint", codes, exps);
+    if (st == DWBNQ_OK) st = check_elem("x", x, dtype);
+    if (st != DWBNQ_OK) return st;
+  }
+  int dev;
+  st = enter_device(device, &dev);
+  if (st != DWBNQ_OK) return st;
+  if (rows == 0 || cols == 0) return DWBNQ_OK;
+  return launch_ckpt8_store(dtype, rows, cols, ld_x, x, codes, exps, static_cast<cudaStream_t>(stream));
+}
+
+int dwbnq_ckpt8_load(int dtype, int64_t rows, int64_t cols, const void *codes, const void *exps, int64_t ld_y, void *y, int device,
+                     void *stream) {
+  clear_error();
+  NvtxRange nvtx_range("dwbnq_ckpt8_load");
+  int st = check_dtype_few_bits(dtype);
+  if (st == DWBNQ_OK) st = check_matrix("y", rows, cols, ld_y);
+  if (st != DWBNQ_OK) return st;
+  if (rows > 0 && cols > 0) {
+    if (!y) return fail(DWBNQ_ERR_INVALID_ARG, "y must not be null");
+    st = check_ckpt8("checkpoint", codes, exps);
+    if (st == DWBNQ_OK) st = check_elem("y", y, dtype);
+    if (st != DWBNQ_OK) return st;
+  }
+  int dev;
+  st = enter_device(device, &dev);
+  if (st != DWBNQ_OK) return st;
+  if (rows == 0 || cols == 0) return DWBNQ_OK;
+  return launch_ckpt8_load(dtype, rows, cols, codes, exps, ld_y, y, static_cast<cudaStream_t>(stream));
+}
+
+int dwbnq_glu_fwd(int dtype, int act, int64_t rows, int64_t cols, int64_t ld_gate, const void *gate, int64_t ld_up, const void *up,
+                  int64_t ld_y, void *y, void *gate_codes, void *gate_exps, void *up_codes, void *up_exps, int device,
+                  void *stream) {
+  clear_error();
+  NvtxRange nvtx_range("dwbnq_glu_fwd");
+  int st = check_dtype_few_bits(dtype);
+  if (st == DWBNQ_OK) st = check_glu_act(act);
+  if (st == DWBNQ_OK) st = check_matrix("gate", rows, cols, ld_gate);
+  if (st == DWBNQ_OK) st = check_matrix("up", rows, cols, ld_up);
+  if (st == DWBNQ_OK) st = check_matrix("y", rows, cols, ld_y);
+  if (st != DWBNQ_OK) return st;
+  if (rows > 0 && cols > 0) {
+    if (!gate || !up || !y) return fail(DWBNQ_ERR_INVALID_ARG, "gate, up and y must not be null");
+    st = check_elem("gate", gate, dtype);
+    if (st == DWBNQ_OK) st = check_elem("up", up, dtype);
+    if (st == DWBNQ_OK) st = check_elem("y", y, dtype);
+    if (st == DWBNQ_OK && (gate_codes || gate_exps || up_codes || up_exps)) {
+      st = check_ckpt8("checkpoint of gate", gate_codes, gate_exps);
+      if (st == DWBNQ_OK) st = check_ckpt8("checkpoint of up", up_codes, up_exps);
+    }
+    if (st != DWBNQ_OK) return st;
+  }
+  int dev;
+  st = enter_device(device, &dev);
+  if (st != DWBNQ_OK) return st;
+  if (rows == 0 || cols == 0) return DWBNQ_OK;
+  return launch_glu_fwd(dtype, act, rows, cols, ld_gate, gate, ld_up, up, ld_y, y, gate_codes, gate_exps, up_codes, up_exps,
+                        static_cast<cudaStream_t>(stream));
+}
+
+int dwbnq_glu_bwd_ckpt8(int dtype, int act, int64_t rows, int64_t cols, const void *gate_codes, const void *gate_exps,
+                        const void *up_codes, const void *up_exps, int64_t ld_dy, const void *dy, int64_t ld_dgate, void *dgate,
+                        int64_t ld_dup, void *dup, void *prod_codes, void *prod_exps, int accum_mask, int device, void *stream) {
+  clear_error();
+  NvtxRange nvtx_range("dwbnq_glu_bwd_ckpt8");
+  int st = check_dtype_few_bits(dtype);
+  if (st == DWBNQ_OK) st = check_glu_act(act);
+  if (st == DWBNQ_OK) st = check_matrix("product", rows, cols, cols);
+  if (st == DWBNQ_OK && (dgate || dup)) st = check_matrix("dy", rows, cols, ld_dy);
+  if (st == DWBNQ_OK && dgate) st = check_matrix("dgate", rows, cols, ld_dgate);
+  if (st == DWBNQ_OK && dup) st = check_matrix("dup", rows, cols, ld_dup);
+  if (st != DWBNQ_OK) return st;
+  if ((prod_codes == nullptr) != (prod_exps == nullptr))
+    return fail(DWBNQ_ERR_INVALID_ARG, "prod_codes and prod_exps must be given together");
+  if (!dgate && !dup && !prod_codes) return DWBNQ_OK;  // nothing to propagate
+  if (rows > 0 && cols > 0) {
+    if ((dgate || dup) && !dy) return fail(DWBNQ_ERR_INVALID_ARG, "dy must not be null");
+    st = check_ckpt8("checkpoint of gate", gate_codes, gate_exps);
+    if (st == DWBNQ_OK) st = check_ckpt8("checkpoint of up", up_codes, up_exps);
+    if (st == DWBNQ_OK && prod_codes) st = check_ckpt8("checkpoint of the product", prod_codes, prod_exps);
+    if (st == DWBNQ_OK) st = check_elem("dy", dy, dtype);
+    if (st == DWBNQ_OK) st = check_elem("dgate", dgate, dtype);
+    if (st == DWBNQ_OK) st = check_elem("dup", dup, dtype);
+    if (st != DWBNQ_OK) return st;
+  }
+  int dev;
+  st = enter_device(device, &dev);
+  if (st != DWBNQ_OK) return st;
+  if (rows == 0 || cols == 0) return DWBNQ_OK;
+  if (!dgate && !dup) dy = nullptr;
+  return launch_glu_bwd(dtype, act, rows, cols, gate_codes, gate_exps, up_codes, up_exps, ld_dy, dy, ld_dgate, dgate, ld_dup, dup,
+                        prod_codes, prod_exps, accum_mask, static_cast<cudaStream_t>(stream));
+}
+
+size_t dwbnq_affine_bwd_workspace_bytes(const dwbnq_affine_desc *desc) {
+  clear_error();
+  return check_affine(desc) == DWBNQ_OK ? affine_bwd_workspace_bytes(*desc) : 0;
+}
+
+int dwbnq_affine_bwd_ckpt8(const dwbnq_affine_desc *desc, const void *codes, const void *exps, const void *dy, void *dw, void *db,
+                           int accum_mask, void *workspace, int device, void *stream) {
+  clear_error();
+  NvtxRange nvtx_range("dwbnq_affine_bwd_ckpt8");
+  int st = check_affine(desc);
+  if (st != DWBNQ_OK) return st;
+  if (desc->c_in == 0) dw = nullptr;
+  if (desc->c_out == 0 || (!dw && !db)) return DWBNQ_OK;  // nothing to propagate
+  if (desc->rows > 0) {
+    if (!dy) return fail(DWBNQ_ERR_INVALID_ARG, "dy must not be null");
+    st = check_elem("dy", dy, desc->dtype);
+    if (st == DWBNQ_OK && dw) st = check_ckpt8("checkpoint of x", codes, exps);
+  }
+  if (st == DWBNQ_OK) st = check_elem("dw", dw, desc->dw_dtype);
+  if (st == DWBNQ_OK) st = check_elem("db", db, desc->dw_dtype);
+  if (st != DWBNQ_OK) return st;
+  if (!workspace) return fail(DWBNQ_ERR_INVALID_ARG, "workspace must not be null");
+  if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(DWBNQ_ERR_INVALID_ARG, "workspace must be 256-byte aligned");
+  int dev;
+  st = enter_device(device, &dev);
+  if (st != DWBNQ_OK) return st;
+  return launch_affine_bwd(*desc, codes, exps, dy, dw, db, accum_mask, workspace, dev, static_cast<cudaStream_t>(stream));
+}
+
+int dwbnq_w4_quantize(int dtype, int32_t c_out, int32_t c_in, int32_t group, int64_t ld_w, const void *w, void *codes, void *scales,
+                      int device, void *stream) {
+  clear_error();
+  NvtxRange nvtx_range("dwbnq_w4_quantize");
+  dwbnq_w4_desc d;
+  std::memset(&d, 0, sizeof(d));
+  d.dtype = dtype; d.group = group; d.c_in = c_in; d.c_out = c_out;
+  int st = check_w4(&d);
+  if (st == DWBNQ_OK) st = check_matrix("w", c_out, c_in, ld_w);
+  if (st != DWBNQ_OK) return st;
+  const bool empty = c_out == 0 || c_in == 0;
+  if (!empty) {
+    if (!w || !codes || !scales) return fail(DWBNQ_ERR_INVALID_ARG, "w, codes and scales must not be null");
+    st = check_elem("w", w, dtype);
+    if (st == DWBNQ_OK) st = check_elem("scales", scales, dtype);
+    if (st != DWBNQ_OK) return st;
+  }
+  int dev;
+  st = enter_device(device, &dev);
+  if (st != DWBNQ_OK) return st;
+  if (empty) return DWBNQ_OK;
+  return launch_w4_quantize(dtype, c_out, c_in, group, ld_w, w, codes, scales, static_cast<cudaStream_t>(stream));
+}
+
+size_t dwbnq_w4_packed_bytes(const dwbnq_w4_desc *desc) {
+  clear_error();
+  return check_w4(desc) == DWBNQ_OK ? w4_packed_bytes(*desc) : 0;
+}
+
+int dwbnq_w4_pack(const dwbnq_w4_desc *desc, const void *codes, const void *scales, const void *zeros, void *packed, int device,
+                  void *stream) {
+  clear_error();
+  NvtxRange nvtx_range("dwbnq_w4_pack");
+  int st = check_w4(desc);
+  if (st != DWBNQ_OK) return st;
+  const bool empty = desc->c_out == 0 || desc->c_in == 0;
+  if (!empty) {
+    if (!codes || !scales || !packed) return fail(DWBNQ_ERR_INVALID_ARG, "codes, scales and packed must not be null");
+    if (desc->has_zeros ? !zeros : zeros != nullptr)
+      return fail(DWBNQ_ERR_INVALID_ARG, "zeros must be given exactly when the desc has zero points");
+    if (reinterpret_cast<uintptr_t>(packed) % 256) return fail(DWBNQ_ERR_INVALID_ARG, "packed must be 256-byte aligned");
+    st = check_elem("scales", scales, desc->dtype);
+    if (st != DWBNQ_OK) return st;
+  }
+  int dev;
+  st = enter_device(device, &dev);
+  if (st != DWBNQ_OK) return st;
+  if (empty) return DWBNQ_OK;
+  return launch_w4_pack(*desc, codes, scales, zeros, packed, static_cast<cudaStream_t>(stream));
+}
+
+int dwbnq_w4_affine_fwd(const dwbnq_w4_desc *desc, int64_t rows, int64_t ld_x, const void *x, const void *packed, const void *b,
+                        int64_t ld_y, void *y, int device, void *stream) {
+  clear_error();
+  NvtxRange nvtx_range("dwbnq_w4_affine_fwd");
+  int st = check_w4(desc);
+  if (st == DWBNQ_OK) st = check_matrix("x", rows, desc->c_in, ld_x);
+  if (st == DWBNQ_OK) st = check_matrix("y", rows, desc->c_out, ld_y);
+  if (st != DWBNQ_OK) return st;
+  if (rows > 16 * 65535LL) return fail(DWBNQ_ERR_UNSUPPORTED, "%lld rows: at most %d", (long long)rows, 16 * 65535);
+  if (rows > 0 && desc->c_out > 0) {
+    if (!y || (desc->c_in > 0 && (!x || !packed))) return fail(DWBNQ_ERR_INVALID_ARG, "x, packed and y must not be null");
+    if (reinterpret_cast<uintptr_t>(packed) % 256) return fail(DWBNQ_ERR_INVALID_ARG, "packed must be 256-byte aligned");
+    st = check_elem("x", x, desc->dtype);
+    if (st == DWBNQ_OK) st = check_elem("y", y, desc->dtype);
+    if (st == DWBNQ_OK) st = check_elem("b", b, desc->dtype);
+    if (st != DWBNQ_OK) return st;
+  }
+  int dev;
+  st = enter_device(device, &dev);
+  if (st != DWBNQ_OK) return st;
+  if (rows == 0 || desc->c_out == 0) return DWBNQ_OK;
+  return launch_w4_affine(*desc, rows, ld_x, x, packed, b, ld_y, y, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -153,6 +153,28 @@ int launch_pwconv(const dwbnq_pwconv_desc &d, float bn_eps, const dwbnq_quant_de
                   const void *b, const void *beta, const void *gamma, const void *mean, const void *var, void *y,
                   void *workspace, int dev, cudaStream_t stream);
 
+// ---- the affine layer in few bits (ckpt8.cu, glu.cu, affine_bwd.cu, affine_w4.cu) -------------------
+int launch_ckpt8_store(int dtype, long long rows, long long cols, long long ld, const void *x, void *codes, void *exps,
+                       cudaStream_t stream);
+int launch_ckpt8_load(int dtype, long long rows, long long cols, const void *codes, const void *exps, long long ld, void *y,
+                      cudaStream_t stream);
+int launch_glu_fwd(int dtype, int act, long long rows, long long cols, long long ld_gate, const void *gate, long long ld_up,
+                   const void *up, long long ld_y, void *y, void *gate_codes, void *gate_exps, void *up_codes, void *up_exps,
+                   cudaStream_t stream);
+int launch_glu_bwd(int dtype, int act, long long rows, long long cols, const void *gate_codes, const void *gate_exps,
+                   const void *up_codes, const void *up_exps, long long ld_dy, const void *dy, long long ld_dgate, void *dgate,
+                   long long ld_dup, void *dup, void *prod_codes, void *prod_exps, int accum, cudaStream_t stream);
+size_t affine_bwd_workspace_bytes(const dwbnq_affine_desc &d);
+int launch_affine_bwd(const dwbnq_affine_desc &d, const void *codes, const void *exps, const void *dy, void *dw, void *db,
+                      int accum_mask, void *workspace, int dev, cudaStream_t stream);
+size_t w4_packed_bytes(const dwbnq_w4_desc &d);
+int launch_w4_quantize(int dtype, int c_out, int c_in, int group, long long ld, const void *w, void *codes, void *scales,
+                       cudaStream_t stream);
+int launch_w4_pack(const dwbnq_w4_desc &d, const void *codes, const void *scales, const void *zeros, void *packed,
+                   cudaStream_t stream);
+int launch_w4_affine(const dwbnq_w4_desc &d, long long rows, long long ld_x, const void *x, const void *packed, const void *b,
+                     long long ld_y, void *y, cudaStream_t stream);
+
 // ---- communicator (comm.cpp) --------------------------------------------------------------
 int comm_allreduce_max(void *comm, float *buf, long long count, cudaStream_t stream,
                        int timeout_ms);

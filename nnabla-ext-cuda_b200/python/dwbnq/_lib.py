@@ -11,7 +11,7 @@ _PKG_ROOT = os.path.abspath(os.path.join(os.path.dirname(__file__), "..", ".."))
 LIB_PATH = os.environ.get("DWBNQ_LIBRARY") or os.path.join(_PKG_ROOT, "libdwbnq.so")
 
 OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_CUDA, ERR_NCCL, ERR_TIMEOUT, ERR_DEVICE_FLAG = range(7)
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2
 Q_NONE, Q_FPQ, Q_POW2, Q_MINMAX = 0, 1, 2, 3
 PATH_AUTO, PATH_GENERIC, PATH_COOP, PATH_TMA, PATH_RAW, PATH_PLANE, PATH_PLANE_GEN = -1, 0, 1, 2, 3, 4, 5
 UNIQUE_ID_BYTES = 128
@@ -45,11 +45,21 @@ class PwConvDesc(ctypes.Structure):
 
 
 PW_MATH_FP32, PW_MATH_TF32 = 0, 1
-ACT_NONE, ACT_RELU, ACT_RELU6 = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_RELU6, ACT_SILU, ACT_GELU = 0, 1, 2, 3, 4
 
 
 class Code8Desc(ctypes.Structure):
     _fields_ = [("in_signed", ctypes.c_int32), ("in_delta", ctypes.c_float)]
+
+
+class AffineDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("dw_dtype", ctypes.c_int32), ("rows", ctypes.c_int64),
+                ("c_in", ctypes.c_int32), ("c_out", ctypes.c_int32), ("ld_dy", ctypes.c_int64)]
+
+
+class W4Desc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("group", ctypes.c_int32), ("c_in", ctypes.c_int32),
+                ("c_out", ctypes.c_int32), ("has_zeros", ctypes.c_int32)]
 
 
 ROUND_HALF_AWAY_FROM_ZERO, ROUND_HALF_TO_EVEN = 0, 1
@@ -106,6 +116,17 @@ SIGNATURES = {
                                 _P(_i64), _P(_int)]),
     "dwbnq_set_forced_path": (_int, [_int]),
     "dwbnq_set_tuning": (_int, [_int, _int, _int, _int]),
+    "dwbnq_ckpt8_store": (_int, [_int, _i64, _i64, _i64, _vp, _vp, _vp, _int, _vp]),
+    "dwbnq_ckpt8_load": (_int, [_int, _i64, _i64, _vp, _vp, _i64, _vp, _int, _vp]),
+    "dwbnq_glu_fwd": (_int, [_int, _int, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _int, _vp]),
+    "dwbnq_glu_bwd_ckpt8": (_int, [_int, _int, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp,
+                                   _int, _int, _vp]),
+    "dwbnq_affine_bwd_workspace_bytes": (ctypes.c_size_t, [_P(AffineDesc)]),
+    "dwbnq_affine_bwd_ckpt8": (_int, [_P(AffineDesc), _vp, _vp, _vp, _vp, _vp, _int, _vp, _int, _vp]),
+    "dwbnq_w4_quantize": (_int, [_int, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _i64, _vp, _vp, _vp, _int, _vp]),
+    "dwbnq_w4_packed_bytes": (ctypes.c_size_t, [_P(W4Desc)]),
+    "dwbnq_w4_pack": (_int, [_P(W4Desc), _vp, _vp, _vp, _vp, _int, _vp]),
+    "dwbnq_w4_affine_fwd": (_int, [_P(W4Desc), _i64, _i64, _vp, _vp, _vp, _i64, _vp, _int, _vp]),
     "dwbnq_comm_get_unique_id": (_int, [_vp]),
     "dwbnq_comm_create": (_int, [_vp, _int, _int, _int, _P(_vp)]),
     "dwbnq_comm_destroy": (_int, [_vp]),

@@ -313,6 +313,284 @@ def fused_dw_bn_quant_code8(x_codes, in_delta, w, b, beta, gamma, mean, variance
     return y
 
 
+# ---- the affine layer of a transformer in few bits ----------------------------------------------
+# 8-bit activation checkpoints with the backward passes that read them, and 4-bit weights. These
+# take float32, float16 and bfloat16 tensors [..., channels] whose last axis is contiguous; the leading
+# axes are rows and may have any one stride (the halves of a wider tensor, a padded buffer).
+
+_FEW_BITS_TYPES = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}
+_GLU_ACTS = {"silu": L.ACT_SILU, "gelu": L.ACT_GELU, "relu": L.ACT_RELU}
+CODE8_GROUP = 32
+
+
+def _few_bits_code(dtype):
+    if dtype not in _FEW_BITS_TYPES:
+        raise TypeError("the few-bit affine operators take float32, float16 and bfloat16 tensors, got %s" % dtype)
+    return _FEW_BITS_TYPES[dtype]
+
+
+def _one_device(*ts):
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("dwbnq operators take CUDA tensors (there is no CPU fallback)")
+        if dev is not None and t.device != dev:
+            raise ValueError("all tensors must live on one device")
+        dev = t.device
+    return dev
+
+
+def _rows_view(t, name):
+    """(rows, cols, row stride) of [..., cols] seen as a matrix."""
+    if t.dim() < 1:
+        raise ValueError("%s must have at least one axis" % name)
+    cols = int(t.shape[-1])
+    rows = 1
+    for s in t.shape[:-1]:
+        rows *= int(s)
+    if cols > 1 and rows > 0 and t.stride(-1) != 1:
+        raise ValueError("%s: the last axis must be contiguous" % name)
+    ld = None  # stride of the innermost leading axis that is longer than 1; the outer ones must continue it
+    span = 1
+    for s, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if s == 1:
+            continue
+        if ld is None:
+            ld = int(st)
+        elif rows > 0 and st != ld * span:
+            raise ValueError("%s: the leading axes must be one run of rows with one stride" % name)
+        span *= int(s)
+    if ld is None or rows == 0:
+        ld = cols
+    if rows > 1 and ld < cols:
+        raise ValueError("%s: rows overlap (stride %d below %d columns)" % (name, ld, cols))
+    return rows, cols, max(ld, cols)
+
+
+def _like(t, name, shape, dtype, device, written=False):
+    """A given output (or a second input) checked against what it has to be; a new one when it is None."""
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+        raise ValueError("%s must be %s of shape %s, got %s of shape %s" % (name, dtype, tuple(shape), t.dtype, tuple(t.shape)))
+    return t
+
+
+class Code8Checkpoint:
+    """A tensor kept in 8 bits: int8 ``codes`` [rows, 32 * groups], uint8 ``exponents`` [rows, groups], the tensor's
+    ``shape`` and ``dtype``. Value = code * 2^(exponent - 133), NaN where the exponent is 255."""
+
+    def __init__(self, codes, exponents, shape, dtype):
+        shape = tuple(int(s) for s in shape)
+        if not shape:
+            raise ValueError("a checkpoint has at least one axis")
+        rows = 1
+        for s in shape[:-1]:
+            rows *= s
+        groups = (shape[-1] + CODE8_GROUP - 1) // CODE8_GROUP
+        if codes.dtype != torch.int8 or tuple(codes.shape) != (rows, CODE8_GROUP * groups) or not codes.is_contiguous():
+            raise ValueError("codes must be contiguous int8 of shape %s" % ((rows, CODE8_GROUP * groups),))
+        if exponents.dtype != torch.uint8 or tuple(exponents.shape) != (rows, groups) or not exponents.is_contiguous():
+            raise ValueError("exponents must be contiguous uint8 of shape %s" % ((rows, groups),))
+        _few_bits_code(dtype)
+        self.codes, self.exponents, self.shape, self.dtype, self.rows, self.cols = codes, exponents, shape, dtype, rows, shape[-1]
+
+    @classmethod
+    def empty(cls, shape, dtype, device):
+        shape = tuple(int(s) for s in shape)
+        rows = 1
+        for s in shape[:-1]:
+            rows *= s
+        groups = (shape[-1] + CODE8_GROUP - 1) // CODE8_GROUP
+        return cls(torch.empty((rows, CODE8_GROUP * groups), dtype=torch.int8, device=device),
+                   torch.empty((rows, groups), dtype=torch.uint8, device=device), shape, dtype)
+
+
+def _ck_out(ck, name, shape, dtype, device):
+    if ck is None:
+        return Code8Checkpoint.empty(shape, dtype, device)
+    if ck.shape != tuple(shape) or ck.dtype != dtype:
+        raise ValueError("%s must be a checkpoint of a %s tensor of shape %s" % (name, dtype, tuple(shape)))
+    return ck
+
+
+def checkpoint_code8(x, out=None):
+    """The 8-bit checkpoint of x [..., channels] (groups of 32 channels share a power-of-two step)."""
+    code = _few_bits_code(x.dtype)
+    ck = _ck_out(out, "out", x.shape, x.dtype, x.device)
+    dev = _one_device(x, ck.codes, ck.exponents)
+    rows, cols, ld = _rows_view(x, "x")
+    with torch.cuda.device(dev):
+        L.check(L.lib().dwbnq_ckpt8_store(code, rows, cols, ld, _ptr(x), _ptr(ck.codes), _ptr(ck.exponents), dev.index,
+                                          _stream(dev)))
+    return ck
+
+
+def restore_code8(ck, dtype=None, out=None):
+    """The values a checkpoint stands for, in the checkpointed tensor's type or ``dtype``."""
+    y = _like(out, "out", ck.shape, out.dtype if out is not None and dtype is None else dtype or ck.dtype, ck.codes.device)
+    code = _few_bits_code(y.dtype)
+    dev = _one_device(ck.codes, ck.exponents, y)
+    rows, cols, ld = _rows_view(y, "out")
+    with torch.cuda.device(dev):
+        L.check(L.lib().dwbnq_ckpt8_load(code, rows, cols, _ptr(ck.codes), _ptr(ck.exponents), ld, _ptr(y), dev.index,
+                                         _stream(dev)))
+    return y
+
+
+def glu(gate, up, act="silu", checkpoint=False, out=None):
+    """act(gate) * up, act one of "silu", "gelu" (erf form) and "relu". With ``checkpoint`` the result is (y,
+    checkpoint of gate, checkpoint of up), all written in one pass. ``out`` may be ``gate`` or ``up``."""
+    code = _few_bits_code(gate.dtype)
+    _like(up, "up", gate.shape, gate.dtype, gate.device)
+    y = _like(out, "out", gate.shape, gate.dtype, gate.device)
+    cks = [Code8Checkpoint.empty(gate.shape, gate.dtype, gate.device) for _ in range(2)] if checkpoint else []
+    dev = _one_device(gate, up, y)
+    (rows, cols, ldg), (_, _, ldu), (_, _, ldy) = _rows_view(gate, "gate"), _rows_view(up, "up"), _rows_view(y, "out")
+    ptrs = [p for ck in cks for p in (_ptr(ck.codes), _ptr(ck.exponents))] or [None] * 4
+    with torch.cuda.device(dev):
+        L.check(L.lib().dwbnq_glu_fwd(code, _GLU_ACTS[act], rows, cols, ldg, _ptr(gate), ldu, _ptr(up), ldy, _ptr(y), *ptrs,
+                                      dev.index, _stream(dev)))
+    return (y, cks[0], cks[1]) if checkpoint else y
+
+
+def glu_backward(ck_gate, ck_up, dy, act="silu", product=False, dgate=None, dup=None, need=(True, True),
+                 accum=(False, False)):
+    """Gradients of glu from the checkpoints of its inputs: (dgate, dup), None where ``need`` is False; with
+    ``product`` also the checkpoint of act(gate) * up, the input of the layer behind. ``accum[i]`` adds onto
+    the given tensor. dgate / dup may be views with a row stride, and either may be ``dy`` itself."""
+    if ck_gate.shape != ck_up.shape or ck_gate.dtype != ck_up.dtype:
+        raise ValueError("the checkpoints of gate and up must have one shape and type")
+    if any(a and n and t is None for a, n, t in zip(accum, need, (dgate, dup))):
+        raise ValueError("accumulating needs the tensor to accumulate onto")
+    shape, dtype = ck_gate.shape, ck_gate.dtype
+    code = _few_bits_code(dtype)
+    device = ck_gate.codes.device
+    if dy is None and (need[0] or need[1]):
+        raise ValueError("dy is needed for dgate and dup")
+    if dy is not None:
+        _like(dy, "dy", shape, dtype, device)
+    dgate = _like(dgate, "dgate", shape, dtype, device) if need[0] else None
+    dup = _like(dup, "dup", shape, dtype, device) if need[1] else None
+    ck = Code8Checkpoint.empty(shape, dtype, device) if product else None
+    dev = _one_device(ck_gate.codes, ck_gate.exponents, ck_up.codes, ck_up.exponents, dy, dgate, dup)
+    rows, cols = ck_gate.rows, ck_gate.cols
+    ld = [_rows_view(t, n)[2] if t is not None else cols for t, n in ((dy, "dy"), (dgate, "dgate"), (dup, "dup"))]
+    mask = (1 if accum[0] else 0) | (2 if accum[1] else 0)
+    with torch.cuda.device(dev):
+        L.check(L.lib().dwbnq_glu_bwd_ckpt8(code, _GLU_ACTS[act], rows, cols, _ptr(ck_gate.codes), _ptr(ck_gate.exponents),
+                                            _ptr(ck_up.codes), _ptr(ck_up.exponents), ld[0], _ptr(dy), ld[1], _ptr(dgate),
+                                            ld[2], _ptr(dup), _ptr(ck.codes) if ck else None,
+                                            _ptr(ck.exponents) if ck else None, mask, dev.index, _stream(dev)))
+    return (dgate, dup, ck) if product else (dgate, dup)
+
+
+def affine_workspace(desc, device):
+    """A workspace tensor of the size affine_weight_backward asks for (``desc``: AffineDesc)."""
+    return torch.empty(int(L.lib().dwbnq_affine_bwd_workspace_bytes(ctypes.byref(desc))), dtype=torch.uint8, device=device)
+
+
+def affine_weight_backward(ck_x, dy, dw=None, db=None, need=(True, True), accum=(False, False), dtype=None, ws=None):
+    """Weight and bias gradients (dw [c_out, c_in], db [c_out]) of an affine layer y = x w^T + b from the checkpoint
+    of x [..., c_in] and dy [..., c_out]; None where ``need`` is False. They have dy's type, or float32 when
+    ``dtype`` (or the given dw / db) says so; ``accum[i]`` adds onto the given tensor."""
+    code = _few_bits_code(dy.dtype)
+    if ck_x.shape[:-1] != tuple(dy.shape[:-1]):
+        raise ValueError("dy %s has other rows than the checkpoint %s" % (tuple(dy.shape), ck_x.shape))
+    if any(a and n and t is None for a, n, t in zip(accum, need, (dw, db))):
+        raise ValueError("accumulating needs the tensor to accumulate onto")
+    if dtype is None:
+        dtype = dw.dtype if dw is not None else db.dtype if db is not None else dy.dtype
+    rows, c_out, ld = _rows_view(dy, "dy")
+    c_in = ck_x.cols
+    dw = _like(dw, "dw", (c_out, c_in), dtype, dy.device) if need[0] else None
+    db = _like(db, "db", (c_out,), dtype, dy.device) if need[1] else None
+    for t, n in ((dw, "dw"), (db, "db")):
+        if t is not None and not t.is_contiguous():
+            raise ValueError("%s must be contiguous" % n)
+    dev = _one_device(dy, ck_x.codes, ck_x.exponents, dw, db, ws)
+    d = L.AffineDesc(dtype=code, dw_dtype=_few_bits_code(dtype), rows=rows, c_in=c_in, c_out=c_out, ld_dy=ld)
+    mask = (2 if accum[0] else 0) | (4 if accum[1] else 0)
+    with torch.cuda.device(dev):
+        if ws is None:
+            ws = affine_workspace(d, dev)
+        elif ws.numel() * ws.element_size() < int(L.lib().dwbnq_affine_bwd_workspace_bytes(ctypes.byref(d))):
+            raise ValueError("ws is smaller than dwbnq_affine_bwd_workspace_bytes asks for")
+        L.check(L.lib().dwbnq_affine_bwd_ckpt8(ctypes.byref(d), _ptr(ck_x.codes), _ptr(ck_x.exponents), _ptr(dy), _ptr(dw),
+                                               _ptr(db), mask, _ptr(ws), dev.index, _stream(dev)))
+    return dw, db
+
+
+class W4Weight:
+    """4-bit weights [c_out, c_in] laid out for affine_w4 (``packed``), with the type of the layer's tensors."""
+
+    def __init__(self, packed, c_out, c_in, group, dtype, has_zeros):
+        self.packed, self.c_out, self.c_in, self.group, self.dtype, self.has_zeros = packed, c_out, c_in, group, dtype, has_zeros
+
+    def desc(self):
+        return L.W4Desc(dtype=_few_bits_code(self.dtype), group=self.group, c_in=self.c_in, c_out=self.c_out,
+                        has_zeros=int(self.has_zeros))
+
+
+def quantize_w4(w, group=128):
+    """Round-to-nearest 4-bit weights of w [c_out, c_in]: (codes uint8 [c_out, c_in] in 0..15, scales [c_out, groups]);
+    the weight is (code - 8) * scale. Lay them out with pack_w4."""
+    if w.dim() != 2:
+        raise ValueError("w must be [c_out, c_in]")
+    code = _few_bits_code(w.dtype)
+    dev = _one_device(w)
+    c_out, c_in, ld = _rows_view(w, "w")
+    codes = torch.empty((c_out, c_in), dtype=torch.uint8, device=dev)
+    scales = torch.empty((c_out, (c_in + group - 1) // group), dtype=w.dtype, device=dev)
+    with torch.cuda.device(dev):
+        L.check(L.lib().dwbnq_w4_quantize(code, c_out, c_in, group, ld, _ptr(w), _ptr(codes), _ptr(scales), dev.index,
+                                          _stream(dev)))
+    return codes, scales
+
+
+def pack_w4(codes, scales, zeros=None, group=128):
+    """Lays 4-bit weights out for affine_w4, once per layer: codes uint8 [c_out, c_in] (0..15), scales [c_out, groups] of
+    the layer's type, zeros uint8 [c_out, groups] or None (8 everywhere); weight = (code - zero) * scale."""
+    if codes.dim() != 2 or codes.dtype != torch.uint8:
+        raise ValueError("codes must be uint8 [c_out, c_in]")
+    c_out, c_in = (int(s) for s in codes.shape)
+    groups = (c_in + group - 1) // group
+    dev = _one_device(codes, scales, zeros)
+    _like(scales, "scales", (c_out, groups), scales.dtype, dev)
+    if zeros is not None:
+        _like(zeros, "zeros", (c_out, groups), torch.uint8, dev)
+    if not all(t is None or t.is_contiguous() for t in (codes, scales, zeros)):
+        raise ValueError("codes, scales and zeros must be contiguous")
+    w4 = W4Weight(None, c_out, c_in, int(group), scales.dtype, zeros is not None)
+    d = w4.desc()
+    with torch.cuda.device(dev):
+        w4.packed = torch.empty(int(L.lib().dwbnq_w4_packed_bytes(ctypes.byref(d))), dtype=torch.uint8, device=dev)
+        L.check(L.lib().dwbnq_w4_pack(ctypes.byref(d), _ptr(codes), _ptr(scales), _ptr(zeros), _ptr(w4.packed), dev.index,
+                                      _stream(dev)))
+    return w4
+
+
+def affine_w4(x, w4, b=None, out=None):
+    """x w^T + b with 4-bit weights, for a few rows (the weights are read once per 16 rows): x [..., c_in]."""
+    if x.dtype != w4.dtype:
+        raise TypeError("x is %s, the weights' scales are %s" % (x.dtype, w4.dtype))
+    rows, c_in, ldx = _rows_view(x, "x")
+    if c_in != w4.c_in:
+        raise ValueError("x has %d channels, the weights %d" % (c_in, w4.c_in))
+    y = _like(out, "out", tuple(x.shape[:-1]) + (w4.c_out,), x.dtype, x.device)
+    if b is not None and not _like(b, "b", (w4.c_out,), x.dtype, x.device).is_contiguous():
+        raise ValueError("b must be contiguous")
+    dev = _one_device(x, w4.packed, b, y)
+    _, _, ldy = _rows_view(y, "out")
+    d = w4.desc()
+    with torch.cuda.device(dev):
+        L.check(L.lib().dwbnq_w4_affine_fwd(ctypes.byref(d), rows, ldx, _ptr(x), _ptr(w4.packed), _ptr(b), ldy, _ptr(y),
+                                            dev.index, _stream(dev)))
+    return y
+
+
 _ACTS = {None: L.ACT_NONE, "none": L.ACT_NONE, "relu": L.ACT_RELU, "relu6": L.ACT_RELU6}
 _MATHS = {"fp32": L.PW_MATH_FP32, "tf32": L.PW_MATH_TF32}
 
