@@ -1,102 +1,626 @@
 // Weight and bias gradients of an affine layer whose input was kept as an 8-bit checkpoint:
 //   dw[o][i] = sum_t dy[t][o] * x[t][i],   db[o] = sum_t dy[t][o],   x[t][i] = code * 2^(b - 133).
+//
+// The weight gradient is a product contracted over the tokens, D[i][o] = X^T dY, on the 5th-generation
+// tensor cores (tcgen05.mma.kind::f16, both factors bfloat16, fp32 accumulators in tensor memory):
+//  * the value of a checkpoint is exact in bfloat16, and so is every product; dy is taken as it is
+//    (bfloat16), or as the exact sum of two (float16) or three (float32) bfloat16 parts, one pass each;
+//  * the 128 accumulator rows are input channels and the columns output channels: a warp that reads the
+//    accumulator back holds 32 consecutive elements of one row of dw per column, so every store is a
+//    coalesced line and nothing is staged. Both factors are MN-major in shared memory, as they lie in
+//    global memory: no transpose anywhere;
+//  * per CTA (one per SM): warp 0 issues the TMA loads of dy, warp 1 the MMAs, warps 2-9 expand the codes
+//    into the swizzled operand layout (and split dy where it is not bfloat16 or its rows are not multiples of
+//    16 bytes), warps 10-17 read the accumulators back;
+//  * where the result is kept in 32 bits, the accumulator is read back after every kRun chunks of 64 tokens
+//    and the runs are added in fp32 registers: the tensor core's adder does not round to nearest, and
+//    over a long batch its error would be the result's;
+//  * tiles that fill whole waves of the 148 SMs are walked as they are; the tiles of the last, partial wave
+//    are cut along the tokens so that it is full too, and a second kernel adds their parts in a fixed order.
+#include <cstring>
+
 #include "ckpt8.cuh"
 #include "dwbnq_internal.h"
+#include "dwbnq_tc.cuh"
 
 namespace dwbnq {
 
 namespace {
 
-// 64 x 64 outputs per CTA, 4 x 4 per thread, 16 tokens per trip.
-template <typename T, typename TW>
-__global__ void __launch_bounds__(256)
-    affine_dw_kernel(const signed char *__restrict__ codes, const unsigned char *__restrict__ exps, long long rows, int c_in,
-                     int c_out, int groups, const T *__restrict__ dy, long long ld, TW *__restrict__ dw, int accum) {
-  pdl_launch_dependents();
-  pdl_wait_for_predecessor();
-  __shared__ float xs[16][64 + 4], ds[16][64 + 4];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, i0 = blockIdx.x * 64, o0 = blockIdx.y * 64;
-  float acc[4][4] = {};
-  for (long long t0 = 0; t0 < rows; t0 += 16) {
-    for (int e = threadIdx.x; e < 16 * 64; e += 256) {
-      const int t = e >> 6, j = e & 63;
-      const bool in = t0 + t < rows;
-      xs[t][j] = in && i0 + j < c_in ? __fmul_rn((float)codes[(t0 + t) * groups * kCkGroup + i0 + j],
-                                                 ck_step(exps[(t0 + t) * groups + (i0 + j) / kCkGroup]))
-                                     : 0.0f;
-      ds[t][j] = in && o0 + j < c_out ? Elem<T>::to_f32(dy[(t0 + t) * ld + o0 + j]) : 0.0f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < 16; ++t)
-#pragma unroll
-      for (int p = 0; p < 4; ++p)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) acc[p][q] = __fmaf_rn(ds[t][ty * 4 + p], xs[t][tx * 4 + q], acc[p][q]);
-    __syncthreads();
+constexpr int kChunk = 64;        // tokens per pipeline stage
+constexpr int kTileI = 128;       // input channels per tile = TMEM lanes
+constexpr int kRun = 4;           // chunks per accumulator run where the sums are kept in 32 bits
+constexpr int kConvWarps = 8, kFirstEpi = 2 + kConvWarps, kEpiWarps = 8;
+constexpr int kThreads = 32 * (kFirstEpi + kEpiWarps);
+constexpr int kXBytes = kChunk * kTileI * 2;
+constexpr int kMaxStages = 8, kTmemCols = 512, kMaxAcc = 4;
+constexpr int kSmemMax = 227 * 1024;
+constexpr int kPlanSms = 148;     // SMs of a B200: the cut of the last wave does not depend on the device it is asked on
+constexpr int kMaxParts = 2 * kPlanSms;
+
+struct DwArgs {
+  const unsigned char *exps;
+  const void *dy;
+  long long ld, rows;
+  int c_in, c_out, groups;
+  int i_tiles;
+  int chunks;              // ceil(rows / 64)
+  int full, segs, units;   // units 0 .. full-1: whole tiles; then segs parts of every further tile
+  int stages;
+  void *dw;
+  float *parts;            // [unit - full][tile columns][128]
+  int accum;
+  int *flag;
+};
+
+// Which tile and which chunks of tokens unit u is.
+__device__ __forceinline__ void dw_unit(const DwArgs &a, int u, int &tile, int &c0, int &c1) {
+  if (u < a.full) {
+    tile = u;
+    c0 = 0;
+    c1 = a.chunks;
+  } else {
+    const int v = u - a.full, q = v / a.segs, s = v - q * a.segs;
+    tile = a.full + q;
+    c0 = (int)((long long)a.chunks * s / a.segs);
+    c1 = (int)((long long)a.chunks * (s + 1) / a.segs);
   }
-#pragma unroll
-  for (int p = 0; p < 4; ++p)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int o = o0 + ty * 4 + p, i = i0 + tx * 4 + q;
-      if (o >= c_out || i >= c_in) continue;
-      TW *w = dw + (long long)o * c_in + i;
-      *w = Elem<TW>::from_f32(accum ? __fadd_rn(Elem<TW>::to_f32(*w), acc[p][q]) : acc[p][q]);
-    }
 }
 
-// 32 output channels per CTA, warp w sums the rows w, w + 8, ...; the eight sums are added in order.
-template <typename T, typename TW>
-__global__ void __launch_bounds__(256)
-    affine_db_kernel(long long rows, int c_out, const T *__restrict__ dy, long long ld, TW *__restrict__ db, int accum) {
+// Eight codes (two words) as bfloat16 values of step `step2` (the step twice): k = (128 + low seven bits) - (128 or
+// 256 for the sign bit), both exact in bfloat16, then the exact product with a power of two.
+__device__ __forceinline__ unsigned int dw_pair(unsigned int two, __nv_bfloat162 step2) {
+  const unsigned int lo = (two & 0x007f007fu) | 0x43004300u, hi = (two & 0x00800080u) | 0x43004300u;
+  const __nv_bfloat162 k = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&lo), *reinterpret_cast<const __nv_bfloat162 *>(&hi));
+  const __nv_bfloat162 v = __hmul2(k, step2);
+  return *reinterpret_cast<const unsigned int *>(&v);
+}
+__device__ __forceinline__ uint4 dw_expand(uint2 c, unsigned int b) {
+  const unsigned int s = b == kCkNonFinite ? 0x7fc07fc0u : b * 0x00800080u - 0x03000300u;  // (b - 6) << 7, twice
+  const __nv_bfloat162 s2 = *reinterpret_cast<const __nv_bfloat162 *>(&s);
+  uint4 r;
+  r.x = dw_pair(__byte_perm(c.x, 0u, 0x4140), s2);
+  r.y = dw_pair(__byte_perm(c.x, 0u, 0x4342), s2);
+  r.z = dw_pair(__byte_perm(c.y, 0u, 0x4140), s2);
+  r.w = dw_pair(__byte_perm(c.y, 0u, 0x4342), s2);
+  return r;
+}
+
+// The leading bfloat16 of v (truncated) and what is left, exactly; an infinity leaves 0, a NaN stays one.
+__device__ __forceinline__ unsigned int dw_head(float &v) {
+  unsigned int h = __float_as_uint(v) & 0xffff0000u;
+  if ((__float_as_uint(v) & 0x7fffffffu) > 0x7f800000u) h = 0x7fc00000u;
+  v = (h & 0x7f800000u) == 0x7f800000u ? 0.0f : __fsub_rn(v, __uint_as_float(h));
+  return h;
+}
+
+// How dy reaches the tensor cores: by TMA as it is (bfloat16); by TMA into a buffer from which the converters split it (float16,
+// float32); or loaded and split by the converters (rows that are not multiples of 16 bytes, which TMA cannot take).
+enum DyMode : int { DY_TMA = 0, DY_RAW = 1, DY_LOAD = 2 };
+template <typename T> struct DyBox { static constexpr int COLS = 128 / (int)sizeof(T); };  // a box is 64 tokens x 128 bytes
+
+// Eight consecutive elements of a row of dy.
+template <typename T> struct DyVec {
+  uint4 w[8 * (int)sizeof(T) / 16];
+  // elements 8 i .. 8 i + 7 of row r of the boxes at `raw`; zero beyond the tensor, as TMA filled them
+  __device__ __forceinline__ void load_shared(const unsigned char *raw, unsigned int r, int i) {
+    constexpr int PER = DyBox<T>::COLS / 8;  // vectors per box row
+    const uint4 *p = reinterpret_cast<const uint4 *>(raw + (i / PER) * 8192 + r * 128 + (i % PER) * 8 * sizeof(T));
+#pragma unroll
+    for (int k = 0; k < 8 * (int)sizeof(T) / 16; ++k) w[k] = p[k];
+  }
+  // columns col .. col + 7 of a row of global memory; zero from column n on
+  __device__ __forceinline__ void load(const T *row, int col, int n) {
+    T e[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e[j] = col + j < n ? __ldg(row + col + j) : Elem<T>::from_f32(0.0f);
+    memcpy(w, e, sizeof(w));
+  }
+  __device__ __forceinline__ void get(float *v) const {
+    T e[8];
+    memcpy(e, w, sizeof(w));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = Elem<T>::to_f32(e[j]);
+  }
+};
+
+// T: type of dy; TW: type of dw; PARTS: bfloat16 parts of dy; DY: DyMode; BN: output channels per tile; KEEP32: short runs
+// added in registers. A stage holds the expanded codes, the parts of dy, the codes, and dy as it came where it is split.
+template <int PARTS, int BN, bool RAW, int TBYTES> struct DwStage {
+  static constexpr int DYB = kChunk * BN * 2, CODES = kXBytes + PARTS * DYB, RAWAT = CODES + kChunk * kTileI,
+                       BYTES = RAWAT + (RAW ? kChunk * BN * TBYTES : 0);
+};
+template <typename T, typename TW, int PARTS, int DY, int BN, bool KEEP32>
+__global__ void __launch_bounds__(kThreads, 1)
+affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ CUtensorMap tm_codes, const DwArgs a) {
+  using S = DwStage<PARTS, BN, DY == DY_RAW, (int)sizeof(T)>;
+  constexpr int DYB = S::DYB, CODES = S::CODES, RAW = S::RAWAT, STAGE = S::BYTES;
+  constexpr int NACC = KEEP32 ? kTmemCols / BN < kMaxAcc ? kTmemCols / BN : kMaxAcc : 2;
+  constexpr int HALF = BN / 2;                        // columns per epilogue warp
+  static_assert(DY != DY_TMA || PARTS == 1, "dy as it is has one part");
+  static_assert(DY == DY_TMA || BN == 128, "a lane splits eight columns of a row");
+  static_assert(STAGE % 1024 == 0, "swizzle atoms");
+  static_assert(!KEEP32 || HALF <= 64, "a thread keeps its columns in registers");
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ unsigned long long bars[3 * kMaxStages + 2 * kMaxAcc + 1];
+  __shared__ unsigned int tmem_base_s;
+  __shared__ int abort_s;
+  unsigned long long *full = bars, *empty = bars + kMaxStages, *conv = bars + 2 * kMaxStages;
+  unsigned long long *acc_full = bars + 3 * kMaxStages, *acc_empty = acc_full + kMaxAcc, *drained = acc_empty + kMaxAcc;
+  const unsigned int base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char *sm = smem_raw + (base - smem_u32(smem_raw));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+      mbar_init(&conv[s], kConvWarps);
+    }
+    for (int b = 0; b < NACC; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], kEpiWarps);
+    }
+    mbar_init(drained, 1);
+    abort_s = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
   pdl_launch_dependents();
   pdl_wait_for_predecessor();
-  __shared__ float part[8][32];
+  const unsigned int tmem_base = tmem_base_s;
+  volatile int *abort_v = &abort_s;
+
+  if (warp == 0) {
+    // ---- TMA loads: the codes and, where it can take them, dy: boxes of 64 tokens x 128 bytes, zero beyond the tensors. Lane l
+    // issues box l, so a stage is one instruction of the warp ----
+    int s = 0, issued = 0;
+    unsigned int ph = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
+      int tile, c0, c1;
+      dw_unit(a, u, tile, c0, c1);
+      const int ot = tile / a.i_tiles, o0 = ot * BN;
+      const int boxes = DY == DY_LOAD ? 0 : min(BN / DyBox<T>::COLS, (a.c_out - o0 + DyBox<T>::COLS - 1) / DyBox<T>::COLS);
+      const int x = lane == 0 ? (tile - ot * a.i_tiles) * kTileI : o0 + (lane - 1) * DyBox<T>::COLS;
+      const unsigned int off = lane == 0 ? (unsigned)CODES : (DY == DY_RAW ? (unsigned)RAW : (unsigned)kXBytes) + (lane - 1) * 8192u;
+      for (int c = c0; c < c1; ++c) {
+        if (!pw_wait(&empty[s], ph ^ 1u) || *abort_v) { ok = false; break; }
+        if (lane == 0) mbar_expect_tx(&full[s], (boxes + 1) * 8192);
+        __syncwarp();
+        if (lane <= boxes) tma_load_2d(sm + s * STAGE + off, lane == 0 ? &tm_codes : &tm_dy, x, c * kChunk, &full[s]);
+        if (issued < a.stages) ++issued;
+        if (++s == a.stages) { s = 0; ph ^= 1u; }
+      }
+    }
+    if (!ok && lane == 0) {
+      if (!*abort_v) { atomicExch(a.flag, 1); *abort_v = 1; }
+      // the copies in flight land before the CTA gives its shared memory back
+      for (; issued > 0; --issued) {
+        if (--s < 0) { s = a.stages - 1; ph ^= 1u; }
+        pw_wait_lane(&full[s], ph);
+      }
+    }
+  } else if (warp == 1) {
+    // ---- MMAs: one thread ----
+    if (lane == 0) {
+      // fp32 accumulator, bfloat16 factors, both MN-major, M = 128; N is set per tile
+      const unsigned int idesc0 = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | (8u << 24);
+      const unsigned long long dx0 = pw_smem_desc(base, 8192, 1024, 2), dd0 = pw_smem_desc(base + kXBytes, 8192, 1024, 2);
+      int s = 0, b = 0;
+      unsigned int ph = 0, aph = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
+        int tile, c0, c1;
+        dw_unit(a, u, tile, c0, c1);
+        const int o0 = tile / a.i_tiles * BN;
+        const int n = min(BN, (a.c_out - o0 + 15) & ~15);
+        const unsigned int idesc = idesc0 | ((unsigned)(n >> 3) << 17);
+        for (int c = c0; ok && c < c1; ++c) {
+          const bool first = KEEP32 ? (c - c0) % kRun == 0 : c == c0;
+          const bool last = c == c1 - 1 || (KEEP32 && (c - c0) % kRun == kRun - 1);
+          const bool r0 = first ? pw_try_wait(&acc_empty[b], aph ^ 1u) : true;
+          const bool r1 = pw_try_wait(&full[s], ph);
+          const bool r2 = pw_try_wait(&conv[s], ph);
+          if (!r0) ok = pw_wait_lane(&acc_empty[b], aph ^ 1u);
+          if (ok && !r1) ok = pw_wait_lane(&full[s], ph);
+          if (ok && !r2) ok = pw_wait_lane(&conv[s], ph);
+          if (!ok || *abort_v) { ok = false; break; }
+          tc_fence_after();
+          const unsigned long long so = (unsigned long long)(s * STAGE) >> 4;
+          const unsigned int d = tmem_base + b * BN;
+          const int steps = (int)min((long long)kChunk / 16, (a.rows - (long long)c * kChunk + 15) / 16);
+          unsigned int acc = first ? 0u : 1u;
+          // the small parts first: a sum that only grows loses least
+#pragma unroll 1
+          for (int p = PARTS - 1; p >= 0; --p) {
+            const unsigned long long dx = dx0 + so, dd = dd0 + so + (unsigned)(p * (DYB >> 4));
+#pragma unroll
+            for (int j = 0; j < kChunk / 16; ++j) {  // a step is 16 rows of 128 bytes
+              if (j < steps) tc_mma_f16(d, dx + j * 128, dd + j * 128, idesc, acc);
+              acc = 1u;
+            }
+          }
+          tc_commit(&empty[s]);
+          if (last) {
+            tc_commit(&acc_full[b]);
+            if (++b == NACC) { b = 0; aph ^= 1u; }
+          }
+          if (++s == a.stages) { s = 0; ph ^= 1u; }
+        }
+      }
+      if (!ok) {
+        if (!*abort_v) { atomicExch(a.flag, 1); *abort_v = 1; }
+        tc_commit(drained);  // the MMAs in flight end before the tensor memory is given back
+        pw_wait_lane(drained, 0);
+      }
+    }
+  } else if (warp < kFirstEpi) {
+    // ---- converters: warp w has tokens 8 w .. 8 w + 7 of every chunk, a pass is two tokens, a lane eight channels. One byte
+    // load per lane brings the warp's 32 exponents, two chunks ahead; the code is kept short, or the warps that issue the loads
+    // and the MMAs would wait for their instructions ----
+    const int cw = warp - 2, l16 = lane & 15, hi = lane >> 4;
+    const unsigned int row0 = cw * 8 + hi, box = (l16 >> 3) * 8192u;
+    int u_l = blockIdx.x, c_l = 0, c1_l = 0, g_l = 0;  // cursor of the exponents
+    auto locate = [&]() {
+      if (u_l >= a.units) return;
+      int tile;
+      dw_unit(a, u_l, tile, c_l, c1_l);
+      g_l = tile % a.i_tiles * (kTileI / kCkGroup) + (lane & 3);
+    };
+    auto next_exp = [&]() -> unsigned int {
+      unsigned int e = kCkMinExp;
+      if (u_l < a.units) {
+        const long long t = (long long)c_l * kChunk + cw * 8 + (lane >> 2);
+        if (t < a.rows && g_l < a.groups) e = __ldg(a.exps + t * a.groups + g_l);
+        if (++c_l == c1_l) {
+          u_l += gridDim.x;
+          locate();
+        }
+      }
+      return e;
+    };
+    locate();
+    unsigned int e0 = next_exp(), e1 = next_exp();
+    int s = 0;
+    unsigned int ph = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
+      int tile, c0, c1;
+      dw_unit(a, u, tile, c0, c1);
+      const int o = tile / a.i_tiles * BN + l16 * 8;
+#pragma unroll 1
+      for (int c = c0; c < c1; ++c) {
+        const unsigned int e2 = next_exp();
+        if (!pw_wait(&full[s], ph) || *abort_v) { ok = false; break; }
+        unsigned char *st = sm + s * STAGE;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const unsigned int r = row0 + 2 * p;
+          const uint2 code = *reinterpret_cast<const uint2 *>(st + CODES + r * kTileI + l16 * 8);
+          const unsigned int e = __shfl_sync(0xffffffffu, e0, (2 * p + hi) * 4 + (l16 >> 2));
+          *reinterpret_cast<uint4 *>(st + box + r * 128 + (((l16 & 7) ^ (2 * p + hi)) << 4)) = dw_expand(code, e);
+        }
+        if (DY != DY_TMA) {
+#pragma unroll 1
+          for (int p = 0; p < 4; ++p) {
+            const unsigned int r = row0 + 2 * p;
+            const long long t = (long long)c * kChunk + r;
+            DyVec<T> x;
+            if (DY == DY_RAW) x.load_shared(st + RAW, r, l16);
+            else x.load(static_cast<const T *>(a.dy) + t * a.ld, o, t < a.rows ? a.c_out : 0);
+            float v[8];
+            x.get(v);
+            unsigned char *to = st + kXBytes + box + r * 128 + (((l16 & 7) ^ (2 * p + hi)) << 4);
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) {
+              unsigned int w[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const unsigned int lo = dw_head(v[2 * j]), up = dw_head(v[2 * j + 1]);
+                w[j] = (lo >> 16) | up;
+              }
+              *reinterpret_cast<uint4 *>(to + q * DYB) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // visible to the tensor core's reads
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&conv[s]);
+        e0 = e1;
+        e1 = e2;
+        if (++s == a.stages) { s = 0; ph ^= 1u; }
+      }
+    }
+    if (!ok && lane == 0 && !*abort_v) { atomicExch(a.flag, 1); *abort_v = 1; }
+  } else {
+    // ---- epilogue: warp (half, quarter) owns input channels [32 quarter, +32) and half of the columns ----
+    const int quarter = warp & 3, half = (warp - kFirstEpi) >> 2;
+    int b = 0;
+    unsigned int aph = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
+      int tile, c0, c1;
+      dw_unit(a, u, tile, c0, c1);
+      const int ot = tile / a.i_tiles, il = quarter * 32 + lane, i = (tile - ot * a.i_tiles) * kTileI + il;
+      const int o0 = ot * BN + half * HALF, n = min(HALF, a.c_out - o0);  // columns that exist (may be negative)
+      const bool whole = u < a.full;
+      TW *dw = static_cast<TW *>(a.dw) + (long long)o0 * a.c_in + i;
+      float *part = whole ? nullptr : a.parts + ((long long)(u - a.full) * BN + half * HALF) * kTileI + il;
+      const bool i_ok = i < a.c_in;
+      auto store = [&](int col, float v) {
+        if (col >= n) return;
+        if (!whole) {
+          part[col * kTileI] = v;
+        } else if (i_ok) {
+          TW *q = dw + (long long)col * a.c_in;
+          *q = Elem<TW>::from_f32(a.accum ? __fadd_rn(Elem<TW>::to_f32(*q), v) : v);
+        }
+      };
+      const int runs = KEEP32 ? (c1 - c0 + kRun - 1) / kRun : 1;
+      float sum[KEEP32 ? HALF : 1];
+      for (int r = 0; ok && r < runs; ++r) {
+        if (!pw_wait(&acc_full[b], aph) || *abort_v) { ok = false; break; }
+        tc_fence_after();
+        const unsigned int taddr = tmem_base + ((unsigned)(quarter * 32) << 16) + b * BN + half * HALF;
+#pragma unroll
+        for (int q = 0; q < HALF; q += 8) {
+          if (!KEEP32 && q >= n) break;
+          unsigned int acc[8];
+          tc_ld8(taddr + q, acc);
+          tc_ld_wait8(acc);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float v = __uint_as_float(acc[j]);
+            if (KEEP32) sum[q + j] = r ? __fadd_rn(sum[q + j], v) : v;
+            else store(q + j, v);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[b]);
+        if (++b == NACC) { b = 0; aph ^= 1u; }
+      }
+      if (KEEP32 && ok) {
+#pragma unroll
+        for (int q = 0; q < HALF; ++q) store(q, sum[q]);
+      }
+    }
+    if (!ok && lane == 0 && !*abort_v) { atomicExch(a.flag, 1); *abort_v = 1; }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+  }
+}
+
+// dw of the tiles whose tokens were cut into `segs` parts: the parts added in order. CTA = tile x 16 of its columns.
+template <typename TW>
+__global__ void __launch_bounds__(kTileI)
+    affine_dw_join_kernel(const float *__restrict__ parts, int first_tile, int segs, int bn, int i_tiles, int c_in, int c_out,
+                          TW *__restrict__ dw, int accum) {
+  pdl_launch_dependents();
+  pdl_wait_for_predecessor();
+  const int tile = first_tile + blockIdx.x, ot = tile / i_tiles, i = (tile - ot * i_tiles) * kTileI + threadIdx.x;
+  if (i >= c_in) return;
+  const float *p = parts + ((long long)blockIdx.x * segs * bn + blockIdx.y * 16) * kTileI + threadIdx.x;
+#pragma unroll 4
+  for (int n = 0; n < 16; ++n) {
+    const int o = ot * bn + blockIdx.y * 16 + n;
+    if (o >= c_out) return;
+    float s = p[n * kTileI];
+    for (int k = 1; k < segs; ++k) s = __fadd_rn(s, p[((long long)k * bn + n) * kTileI]);
+    TW *q = dw + (long long)o * c_in + i;
+    *q = Elem<TW>::from_f32(accum ? __fadd_rn(Elem<TW>::to_f32(*q), s) : s);
+  }
+}
+
+// ---- bias gradient: CTA (32 channels, slice of the rows), warp w the rows w, w + 8, ...; then the slices in order ----
+constexpr int kDbSlices = 64;
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+    affine_db_kernel(long long rows, int c_out, const T *__restrict__ dy, long long ld, float *__restrict__ part) {
+  pdl_launch_dependents();
+  pdl_wait_for_predecessor();
+  __shared__ float sums[8][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, o = blockIdx.x * 32 + lane;
+  const long long r0 = rows * blockIdx.y / gridDim.y, r1 = rows * (blockIdx.y + 1) / gridDim.y;
   float s = 0.0f;
   if (o < c_out)
-    for (long long t = w; t < rows; t += 8) s = __fadd_rn(s, Elem<T>::to_f32(dy[t * ld + o]));
-  part[w][lane] = s;
+    for (long long t = r0 + w; t < r1; t += 8) s = __fadd_rn(s, Elem<T>::to_f32(dy[t * ld + o]));
+  sums[w][lane] = s;
   __syncthreads();
   if (w || o >= c_out) return;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) s = __fadd_rn(s, part[i][lane]);
+  for (int i = 1; i < 8; ++i) s = __fadd_rn(s, sums[i][lane]);
+  part[(long long)blockIdx.y * c_out + o] = s;
+}
+template <typename TW>
+__global__ void __launch_bounds__(256)
+    affine_db_join_kernel(const float *__restrict__ part, int slices, int c_out, TW *__restrict__ db, int accum) {
+  pdl_launch_dependents();
+  pdl_wait_for_predecessor();
+  const int o = blockIdx.x * 256 + threadIdx.x;
+  if (o >= c_out) return;
+  float s = 0.0f;
+  for (int i = 0; i < slices; ++i) s = __fadd_rn(s, part[(long long)i * c_out + o]);
   db[o] = Elem<TW>::from_f32(accum ? __fadd_rn(Elem<TW>::to_f32(db[o]), s) : s);
 }
 
-template <typename T, typename TW>
+// ---- host side ---------------------------------------------------------------------------------------------
+
+struct DwPlan {
+  int bn, i_tiles, o_tiles, chunks, full, segs, units;
+  size_t parts_bytes, bytes;
+};
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+// `wide`: tiles of 256 output channels. Whole waves of kPlanSms tiles are walked uncut; the R tiles left over are cut into
+// the number of parts that costs least, in chunks of 64 tokens on the busiest SM: ceil(R s / SMs) parts of ceil(chunks / s)
+// chunks, each with about 4 chunks' worth of read-back, and 16 for the second kernel and the parts' traffic.
+DwPlan dw_plan(const dwbnq_affine_desc &d, bool wide) {
+  DwPlan p;
+  p.bn = wide ? 256 : 128;
+  p.i_tiles = (d.c_in + kTileI - 1) / kTileI;
+  p.o_tiles = (d.c_out + p.bn - 1) / p.bn;
+  p.chunks = (int)((d.rows + kChunk - 1) / kChunk);
+  const long long tiles = (long long)p.i_tiles * p.o_tiles;
+  const int rest = (int)(tiles % kPlanSms);
+  p.full = (int)(tiles - rest);
+  p.segs = 1;
+  long long best = 0;
+  for (int s = 1; rest && s <= p.chunks && rest * s <= kMaxParts; ++s) {
+    const long long cost = (long long)((rest * s + kPlanSms - 1) / kPlanSms) * ((p.chunks + s - 1) / s + 4) + (s > 1 ? 16 : 0);
+    if (s == 1 || cost < best) { best = cost; p.segs = s; }
+  }
+  if (p.segs == 1) p.full = (int)tiles;
+  p.units = p.segs == 1 ? (int)tiles : p.full + rest * p.segs;
+  p.parts_bytes = p.segs == 1 ? 0 : up256((size_t)rest * p.segs * p.bn * kTileI * 4);
+  p.bytes = 256 + p.parts_bytes + up256((size_t)kDbSlices * d.c_out * 4);
+  return p;
+}
+bool dw_wide(const dwbnq_affine_desc &d) { return d.dtype == DWBNQ_BF16 && d.dw_dtype == DWBNQ_BF16; }
+
+typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                             const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess) {
+      (void)cudaGetLastError();
+      p = nullptr;
+    }
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+
+template <typename T, typename TW, int PARTS, int DY, int BN, bool KEEP32>
+int launch_dw(const CUtensorMap &tm, const CUtensorMap &tc, DwArgs &a, cudaStream_t stream) {
+  constexpr int STAGE = DwStage<PARTS, BN, DY == DY_RAW, (int)sizeof(T)>::BYTES;
+  constexpr int fit = (kSmemMax - 2048) / STAGE;
+  a.stages = fit < kMaxStages ? fit : kMaxStages;
+  const int smem = a.stages * STAGE + 1024;
+  auto kern = affine_dw_kernel<T, TW, PARTS, DY, BN, KEEP32>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return fail_cuda(e, "affine_dw_kernel attributes");
+  const int sms = sm_count(-1);
+  e = launch_pdl(kern, dim3((unsigned)(a.units < sms ? a.units : sms)), dim3(kThreads), (size_t)smem, stream, tm, tc, a);
+  return e == cudaSuccess ? DWBNQ_OK : fail_cuda(e, "affine_dw_kernel launch");
+}
+
+template <typename TW>
 int run_t(const dwbnq_affine_desc &d, const void *codes, const void *exps, const void *dy, void *dw, void *db, int accum_mask,
-          cudaStream_t stream) {
-  const int groups = (d.c_in + kCkGroup - 1) / kCkGroup;
+          void *workspace, int dev, cudaStream_t stream) {
   cudaError_t e;
+  if (d.rows == 0) {  // sums of nothing
+    if (dw && !(accum_mask & 2) && (e = cudaMemsetAsync(dw, 0, sizeof(TW) * (size_t)d.c_out * d.c_in, stream)) != cudaSuccess)
+      return fail_cuda(e, "cudaMemsetAsync");
+    if (db && !(accum_mask & 4) && (e = cudaMemsetAsync(db, 0, sizeof(TW) * (size_t)d.c_out, stream)) != cudaSuccess)
+      return fail_cuda(e, "cudaMemsetAsync");
+    return DWBNQ_OK;
+  }
+  const int eb = d.dtype == DWBNQ_F32 ? 4 : 2;
+  const bool tma = reinterpret_cast<uintptr_t>(dy) % 16 == 0 && d.ld_dy * eb % 16 == 0 && d.ld_dy < (1LL << 36);
+  const DwPlan p = dw_plan(d, dw_wide(d) && tma);
+  float *parts = reinterpret_cast<float *>(workspace);
+  float *dbp = reinterpret_cast<float *>(static_cast<char *>(workspace) + 256 + p.parts_bytes);
   if (dw) {
-    const dim3 grid((unsigned)((d.c_in + 63) / 64), (unsigned)((d.c_out + 63) / 64));
-    e = launch_pdl(affine_dw_kernel<T, TW>, grid, dim3(256), 0, stream, static_cast<const signed char *>(codes),
-                   static_cast<const unsigned char *>(exps), (long long)d.rows, d.c_in, d.c_out, groups,
-                   static_cast<const T *>(dy), (long long)d.ld_dy, static_cast<TW *>(dw), (accum_mask >> 1) & 1);
-    if (e != cudaSuccess) return fail_cuda(e, "affine_dw_kernel launch");
+    DwArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.exps = static_cast<const unsigned char *>(exps);
+    a.dy = dy;
+    a.ld = d.ld_dy; a.rows = d.rows; a.c_in = d.c_in; a.c_out = d.c_out;
+    a.groups = (d.c_in + kCkGroup - 1) / kCkGroup;
+    a.i_tiles = p.i_tiles; a.chunks = p.chunks; a.full = p.full; a.segs = p.segs; a.units = p.units;
+    a.dw = dw; a.parts = parts; a.accum = (accum_mask >> 1) & 1;
+    int st = device_flag_ptr(dev, &a.flag);
+    if (st != DWBNQ_OK) return st;
+    CUtensorMap tm, tc;
+    std::memset(&tm, 0, sizeof(tm));
+    std::memset(&tc, 0, sizeof(tc));
+    if (!encode_fn()) return fail(DWBNQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint32_t es[2] = {1, 1};
+    const cuuint64_t cdim[2] = {(cuuint64_t)a.groups * kCkGroup, (cuuint64_t)d.rows}, cstr[1] = {cdim[0]};
+    const cuuint32_t cbox[2] = {kTileI, kChunk};
+    CUresult r = encode_fn()(&tc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(codes), cdim, cstr, cbox, es,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(DWBNQ_ERR_CUDA, "cuTensorMapEncodeTiled(codes) failed with CUresult %d", (int)r);
+    if (tma) {
+      const cuuint64_t dim[2] = {(cuuint64_t)d.c_out, (cuuint64_t)d.rows}, str[1] = {(cuuint64_t)d.ld_dy * eb};
+      const cuuint32_t box[2] = {(cuuint32_t)(128 / eb), kChunk};
+      const bool as_is = d.dtype == DWBNQ_BF16;
+      r = encode_fn()(&tm, as_is ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : eb == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                      2, const_cast<void *>(dy), dim, str, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      as_is ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+      if (r != CUDA_SUCCESS) return fail(DWBNQ_ERR_CUDA, "cuTensorMapEncodeTiled(dy) failed with CUresult %d", (int)r);
+    }
+    if constexpr (sizeof(TW) == 4) {
+      if (d.dtype == DWBNQ_F32)
+        st = tma ? launch_dw<float, TW, 3, DY_RAW, 128, true>(tm, tc, a, stream) : launch_dw<float, TW, 3, DY_LOAD, 128, true>(tm, tc, a, stream);
+      else if (d.dtype == DWBNQ_F16)
+        st = tma ? launch_dw<__half, TW, 2, DY_RAW, 128, true>(tm, tc, a, stream) : launch_dw<__half, TW, 2, DY_LOAD, 128, true>(tm, tc, a, stream);
+      else
+        st = tma ? launch_dw<__nv_bfloat16, TW, 1, DY_TMA, 128, true>(tm, tc, a, stream)
+                 : launch_dw<__nv_bfloat16, TW, 1, DY_LOAD, 128, true>(tm, tc, a, stream);
+    } else if constexpr (std::is_same<TW, __half>::value) {
+      st = tma ? launch_dw<__half, TW, 2, DY_RAW, 128, true>(tm, tc, a, stream) : launch_dw<__half, TW, 2, DY_LOAD, 128, true>(tm, tc, a, stream);
+    } else {
+      st = tma ? launch_dw<__nv_bfloat16, TW, 1, DY_TMA, 256, false>(tm, tc, a, stream)
+               : launch_dw<__nv_bfloat16, TW, 1, DY_LOAD, 128, true>(tm, tc, a, stream);
+    }
+    if (st != DWBNQ_OK) return st;
+    if (p.segs > 1) {
+      const dim3 grid((unsigned)((p.units - p.full) / p.segs), (unsigned)(p.bn / 16));
+      e = launch_pdl(affine_dw_join_kernel<TW>, grid, dim3(kTileI), 0, stream, (const float *)parts, p.full, p.segs, p.bn, p.i_tiles,
+                     d.c_in, d.c_out, static_cast<TW *>(dw), (accum_mask >> 1) & 1);
+      if (e != cudaSuccess) return fail_cuda(e, "affine_dw_join_kernel launch");
+    }
   }
   if (db) {
-    e = launch_pdl(affine_db_kernel<T, TW>, dim3((unsigned)((d.c_out + 31) / 32)), dim3(256), 0, stream, (long long)d.rows,
-                   d.c_out, static_cast<const T *>(dy), (long long)d.ld_dy, static_cast<TW *>(db), (accum_mask >> 2) & 1);
+    const int slices = (int)(d.rows < 32 ? 1 : d.rows / 32 < kDbSlices ? d.rows / 32 : kDbSlices);
+    const dim3 grid((unsigned)((d.c_out + 31) / 32), (unsigned)slices);
+    if (d.dtype == DWBNQ_F32)
+      e = launch_pdl(affine_db_kernel<float>, grid, dim3(256), 0, stream, (long long)d.rows, d.c_out, static_cast<const float *>(dy), (long long)d.ld_dy, dbp);
+    else if (d.dtype == DWBNQ_F16)
+      e = launch_pdl(affine_db_kernel<__half>, grid, dim3(256), 0, stream, (long long)d.rows, d.c_out, static_cast<const __half *>(dy), (long long)d.ld_dy, dbp);
+    else
+      e = launch_pdl(affine_db_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, (long long)d.rows, d.c_out, static_cast<const __nv_bfloat16 *>(dy), (long long)d.ld_dy, dbp);
     if (e != cudaSuccess) return fail_cuda(e, "affine_db_kernel launch");
+    e = launch_pdl(affine_db_join_kernel<TW>, dim3((unsigned)((d.c_out + 255) / 256)), dim3(256), 0, stream, (const float *)dbp, slices, d.c_out,
+                   static_cast<TW *>(db), (accum_mask >> 2) & 1);
+    if (e != cudaSuccess) return fail_cuda(e, "affine_db_join_kernel launch");
   }
   return DWBNQ_OK;
 }
 
 }  // namespace
 
-size_t affine_bwd_workspace_bytes(const dwbnq_affine_desc &) { return 256; }
+size_t affine_bwd_workspace_bytes(const dwbnq_affine_desc &d) {
+  const size_t narrow = dw_plan(d, false).bytes, wide = dw_wide(d) ? dw_plan(d, true).bytes : 0;
+  return narrow > wide ? narrow : wide;
+}
 
 int launch_affine_bwd(const dwbnq_affine_desc &d, const void *codes, const void *exps, const void *dy, void *dw, void *db,
-                      int accum_mask, void *, int, cudaStream_t stream) {
-  if (d.dtype == DWBNQ_F32) return run_t<float, float>(d, codes, exps, dy, dw, db, accum_mask, stream);
-  if (d.dtype == DWBNQ_F16)
-    return d.dw_dtype == DWBNQ_F32 ? run_t<__half, float>(d, codes, exps, dy, dw, db, accum_mask, stream)
-                                   : run_t<__half, __half>(d, codes, exps, dy, dw, db, accum_mask, stream);
-  return d.dw_dtype == DWBNQ_F32 ? run_t<__nv_bfloat16, float>(d, codes, exps, dy, dw, db, accum_mask, stream)
-                                 : run_t<__nv_bfloat16, __nv_bfloat16>(d, codes, exps, dy, dw, db, accum_mask, stream);
+                      int accum_mask, void *workspace, int dev, cudaStream_t stream) {
+  if (d.dw_dtype == DWBNQ_F32) return run_t<float>(d, codes, exps, dy, dw, db, accum_mask, workspace, dev, stream);
+  if (d.dw_dtype == DWBNQ_F16) return run_t<__half>(d, codes, exps, dy, dw, db, accum_mask, workspace, dev, stream);
+  return run_t<__nv_bfloat16>(d, codes, exps, dy, dw, db, accum_mask, workspace, dev, stream);
 }
 
 }  // namespace dwbnq

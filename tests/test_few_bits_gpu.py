@@ -286,8 +286,10 @@ def test_affine_gradients_real_values(cuda_device, dt, rows, c_in, c_out):
     assert ((db.cpu().double() - wantb).abs() <= (rows + 8) * 2.0 ** -24 * dy.double().abs().sum(0)).all()
     again, _ = ops.affine_weight_backward(ck, dy.to(cuda_device), dtype=torch.float32)
     assert torch.equal(again, dw)  # the order of the sum is fixed
+    # 16-bit results are summed in longer runs: the first bound, and one rounding
     narrow, _ = ops.affine_weight_backward(ck, dy.to(cuda_device))
-    assert torch.equal(narrow, dw.to(dtype))
+    lim = (rows + 8) * 2.0 ** -23 * size + want.abs() * fb.half_step(dtype) * 1.02
+    assert ((narrow.cpu().double() - want).abs() <= lim).all()
 
 
 def test_affine_gradients_of_nothing(cuda_device):
