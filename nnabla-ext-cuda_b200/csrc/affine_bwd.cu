@@ -9,12 +9,14 @@
 //    accumulator back holds 32 consecutive elements of one row of dw per column, so every store is a
 //    coalesced line and nothing is staged. Both factors are MN-major in shared memory, as they lie in
 //    global memory: no transpose anywhere;
-//  * per CTA (one per SM): warp 0 issues the TMA loads of dy, warp 1 the MMAs, warps 2-9 expand the codes
-//    into the swizzled operand layout (and split dy where it is not bfloat16 or its rows are not multiples of
-//    16 bytes), warps 10-17 read the accumulators back;
-//  * where the result is kept in 32 bits, the accumulator is read back after every kRun chunks of 64 tokens
-//    and the runs are added in fp32 registers: the tensor core's adder does not round to nearest, and
-//    over a long batch its error would be the result's;
+//  * per CTA (one per SM): warp 0 issues the TMA loads, warp 1 the MMAs, warps 2-17 expand the codes into the
+//    swizzled operand layout (and split dy where it is not bfloat16 or its rows are not multiples of 16 bytes),
+//    warps 18-25 read the accumulators back. The converters work in as many groups as there are stages, a
+//    chunk of 64 tokens per group: one warp needs about 1400 cycles from its wait to its next one, and with all
+//    of them on every chunk that was the kernel's pace (512 cycles of MMAs per chunk);
+//  * where the result is kept in 32 bits, the accumulator is read back after a run of a few chunks and the runs
+//    are added to dw in fp32: the tensor core's adder truncates, by 2^-25 of the sum per step of 16 tokens on
+//    average, and over a long batch that would be the result's error;
 //  * tiles that fill whole waves of the 148 SMs are walked as they are; the tiles of the last, partial wave
 //    are cut along the tokens so that it is full too, and a second kernel adds their parts in a fixed order.
 #include <cstring>
@@ -29,11 +31,10 @@ namespace {
 
 constexpr int kChunk = 64;        // tokens per pipeline stage
 constexpr int kTileI = 128;       // input channels per tile = TMEM lanes
-constexpr int kRun = 4;           // chunks per accumulator run where the sums are kept in 32 bits
-constexpr int kConvWarps = 8, kFirstEpi = 2 + kConvWarps, kEpiWarps = 8;
+constexpr int kConvWarps = 16, kFirstEpi = 2 + kConvWarps, kEpiWarps = 8;
 constexpr int kThreads = 32 * (kFirstEpi + kEpiWarps);
 constexpr int kXBytes = kChunk * kTileI * 2;
-constexpr int kMaxStages = 8, kTmemCols = 512, kMaxAcc = 4;
+constexpr int kMaxStages = 4, kTmemCols = 512, kMaxAcc = 4;
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kPlanSms = 148;     // SMs of a B200: the cut of the last wave does not depend on the device it is asked on
 constexpr int kMaxParts = 2 * kPlanSms;
@@ -46,7 +47,6 @@ struct DwArgs {
   int i_tiles;
   int chunks;              // ceil(rows / 64)
   int full, segs, units;   // units 0 .. full-1: whole tiles; then segs parts of every further tile
-  int stages;
   void *dw;
   float *parts;            // [unit - full][tile columns][128]
   int accum;
@@ -124,23 +124,28 @@ template <typename T> struct DyVec {
   }
 };
 
-// T: type of dy; TW: type of dw; PARTS: bfloat16 parts of dy; DY: DyMode; BN: output channels per tile; KEEP32: short runs
-// added in registers. A stage holds the expanded codes, the parts of dy, the codes, and dy as it came where it is split.
-template <int PARTS, int BN, bool RAW, int TBYTES> struct DwStage {
-  static constexpr int DYB = kChunk * BN * 2, CODES = kXBytes + PARTS * DYB, RAWAT = CODES + kChunk * kTileI,
-                       BYTES = RAWAT + (RAW ? kChunk * BN * TBYTES : 0);
+// A stage holds the expanded codes, the parts of dy, the codes, and dy as it came where it is split. Two or four stages: the
+// converters' groups are as many, so that each stage's barriers are always awaited by the same group (a parity wait cannot
+// tell a phase from the one after the next).
+template <int PARTS, int BN, int DY, int TBYTES> struct DwStage {
+  static constexpr int DYB = kChunk * BN * 2, CODES = kXBytes + PARTS * DYB, RAW = CODES + kChunk * kTileI,
+                       BYTES = RAW + (DY == DY_RAW ? kChunk * BN * TBYTES : 0), COUNT = 4 * BYTES + 2048 <= kSmemMax ? 4 : 2;
 };
-template <typename T, typename TW, int PARTS, int DY, int BN, bool KEEP32>
+
+// T: type of dy; TW: type of dw (32 bits: sums in short runs); PARTS: bfloat16 parts of dy; BN: output channels per tile.
+template <typename T, typename TW, int PARTS, int DY, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
 affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ CUtensorMap tm_codes, const DwArgs a) {
-  using S = DwStage<PARTS, BN, DY == DY_RAW, (int)sizeof(T)>;
-  constexpr int DYB = S::DYB, CODES = S::CODES, RAW = S::RAWAT, STAGE = S::BYTES;
-  constexpr int NACC = KEEP32 ? kTmemCols / BN < kMaxAcc ? kTmemCols / BN : kMaxAcc : 2;
+  using S = DwStage<PARTS, BN, DY, (int)sizeof(T)>;
+  constexpr int DYB = S::DYB, STAGE = S::BYTES, STAGES = S::COUNT;
+  constexpr int GROUP = kConvWarps / STAGES, TOKENS = kChunk / GROUP;  // converter warps per group, tokens per warp and chunk
+  constexpr bool KEEP32 = sizeof(TW) == 4;
+  constexpr int RUN = PARTS == 1 ? 16 : PARTS == 2 ? 8 : 4;  // chunks per run: the more digits in dy, the more the adder drops
+  constexpr int NACC = kTmemCols / BN < kMaxAcc ? kTmemCols / BN : kMaxAcc;
   constexpr int HALF = BN / 2;                        // columns per epilogue warp
   static_assert(DY != DY_TMA || PARTS == 1, "dy as it is has one part");
   static_assert(DY == DY_TMA || BN == 128, "a lane splits eight columns of a row");
-  static_assert(STAGE % 1024 == 0, "swizzle atoms");
-  static_assert(!KEEP32 || HALF <= 64, "a thread keeps its columns in registers");
+  static_assert(STAGE % 1024 == 0 && STAGES * STAGE + 2048 <= kSmemMax, "swizzle atoms; shared memory");
   extern __shared__ unsigned char smem_raw[];
   __shared__ unsigned long long bars[3 * kMaxStages + 2 * kMaxAcc + 1];
   __shared__ unsigned int tmem_base_s;
@@ -152,10 +157,10 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < a.stages; ++s) {
+    for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
-      mbar_init(&conv[s], kConvWarps);
+      mbar_init(&conv[s], GROUP);
     }
     for (int b = 0; b < NACC; ++b) {
       mbar_init(&acc_full[b], 1);
@@ -180,165 +185,166 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
   volatile int *abort_v = &abort_s;
 
   if (warp == 0) {
-    // ---- TMA loads: the codes and, where it can take them, dy: boxes of 64 tokens x 128 bytes, zero beyond the tensors. Lane l
-    // issues box l, so a stage is one instruction of the warp ----
+    // ---- TMA loads: the codes and, where it can take them, dy: boxes of 64 tokens x 128 bytes, zero beyond the tensors ----
     int s = 0, issued = 0;
     unsigned int ph = 0;
     bool ok = true;
     for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
       int tile, c0, c1;
       dw_unit(a, u, tile, c0, c1);
-      const int ot = tile / a.i_tiles, o0 = ot * BN;
-      const int boxes = DY == DY_LOAD ? 0 : min(BN / DyBox<T>::COLS, (a.c_out - o0 + DyBox<T>::COLS - 1) / DyBox<T>::COLS);
-      const int x = lane == 0 ? (tile - ot * a.i_tiles) * kTileI : o0 + (lane - 1) * DyBox<T>::COLS;
-      const unsigned int off = lane == 0 ? (unsigned)CODES : (DY == DY_RAW ? (unsigned)RAW : (unsigned)kXBytes) + (lane - 1) * 8192u;
+      const int ot = tile / a.i_tiles, o0 = ot * BN, i0 = (tile - ot * a.i_tiles) * kTileI;
+      constexpr int COLS = DyBox<T>::COLS, MAXBOX = BN / COLS, DYAT = DY == DY_RAW ? S::RAW : kXBytes;
+      const int boxes = DY == DY_LOAD ? 0 : min(MAXBOX, (a.c_out - o0 + COLS - 1) / COLS);
       for (int c = c0; c < c1; ++c) {
         if (!pw_wait(&empty[s], ph ^ 1u) || *abort_v) { ok = false; break; }
-        if (lane == 0) mbar_expect_tx(&full[s], (boxes + 1) * 8192);
+        if (elect_one()) {
+          unsigned char *st = sm + s * STAGE;
+          mbar_expect_tx(&full[s], (boxes + 1) * 8192);
+          tma_load_2d(st + S::CODES, &tm_codes, i0, c * kChunk, &full[s]);
+#pragma unroll
+          for (int q = 0; q < MAXBOX; ++q)
+            if (q < boxes) tma_load_2d(st + DYAT + q * 8192, &tm_dy, o0 + q * COLS, c * kChunk, &full[s]);
+        }
         __syncwarp();
-        if (lane <= boxes) tma_load_2d(sm + s * STAGE + off, lane == 0 ? &tm_codes : &tm_dy, x, c * kChunk, &full[s]);
-        if (issued < a.stages) ++issued;
-        if (++s == a.stages) { s = 0; ph ^= 1u; }
+        if (issued < STAGES) ++issued;
+        if (++s == STAGES) { s = 0; ph ^= 1u; }
       }
     }
     if (!ok && lane == 0) {
       if (!*abort_v) { atomicExch(a.flag, 1); *abort_v = 1; }
       // the copies in flight land before the CTA gives its shared memory back
       for (; issued > 0; --issued) {
-        if (--s < 0) { s = a.stages - 1; ph ^= 1u; }
+        if (--s < 0) { s = STAGES - 1; ph ^= 1u; }
         pw_wait_lane(&full[s], ph);
       }
     }
   } else if (warp == 1) {
-    // ---- MMAs: one thread ----
-    if (lane == 0) {
-      // fp32 accumulator, bfloat16 factors, both MN-major, M = 128; N is set per tile
-      const unsigned int idesc0 = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | (8u << 24);
-      const unsigned long long dx0 = pw_smem_desc(base, 8192, 1024, 2), dd0 = pw_smem_desc(base + kXBytes, 8192, 1024, 2);
-      int s = 0, b = 0;
-      unsigned int ph = 0, aph = 0;
-      bool ok = true;
-      for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
-        int tile, c0, c1;
-        dw_unit(a, u, tile, c0, c1);
-        const int o0 = tile / a.i_tiles * BN;
-        const int n = min(BN, (a.c_out - o0 + 15) & ~15);
-        const unsigned int idesc = idesc0 | ((unsigned)(n >> 3) << 17);
-        for (int c = c0; ok && c < c1; ++c) {
-          const bool first = KEEP32 ? (c - c0) % kRun == 0 : c == c0;
-          const bool last = c == c1 - 1 || (KEEP32 && (c - c0) % kRun == kRun - 1);
-          const bool r0 = first ? pw_try_wait(&acc_empty[b], aph ^ 1u) : true;
-          const bool r1 = pw_try_wait(&full[s], ph);
-          const bool r2 = pw_try_wait(&conv[s], ph);
-          if (!r0) ok = pw_wait_lane(&acc_empty[b], aph ^ 1u);
-          if (ok && !r1) ok = pw_wait_lane(&full[s], ph);
-          if (ok && !r2) ok = pw_wait_lane(&conv[s], ph);
-          if (!ok || *abort_v) { ok = false; break; }
-          tc_fence_after();
-          const unsigned long long so = (unsigned long long)(s * STAGE) >> 4;
-          const unsigned int d = tmem_base + b * BN;
-          const int steps = (int)min((long long)kChunk / 16, (a.rows - (long long)c * kChunk + 15) / 16);
-          unsigned int acc = first ? 0u : 1u;
-          // the small parts first: a sum that only grows loses least
-#pragma unroll 1
-          for (int p = PARTS - 1; p >= 0; --p) {
-            const unsigned long long dx = dx0 + so, dd = dd0 + so + (unsigned)(p * (DYB >> 4));
-#pragma unroll
-            for (int j = 0; j < kChunk / 16; ++j) {  // a step is 16 rows of 128 bytes
-              if (j < steps) tc_mma_f16(d, dx + j * 128, dd + j * 128, idesc, acc);
-              acc = 1u;
-            }
-          }
-          tc_commit(&empty[s]);
-          if (last) {
-            tc_commit(&acc_full[b]);
-            if (++b == NACC) { b = 0; aph ^= 1u; }
-          }
-          if (++s == a.stages) { s = 0; ph ^= 1u; }
-        }
-      }
-      if (!ok) {
-        if (!*abort_v) { atomicExch(a.flag, 1); *abort_v = 1; }
-        tc_commit(drained);  // the MMAs in flight end before the tensor memory is given back
-        pw_wait_lane(drained, 0);
-      }
-    }
-  } else if (warp < kFirstEpi) {
-    // ---- converters: warp w has tokens 8 w .. 8 w + 7 of every chunk, a pass is two tokens, a lane eight channels. One byte
-    // load per lane brings the warp's 32 exponents, two chunks ahead; the code is kept short, or the warps that issue the loads
-    // and the MMAs would wait for their instructions ----
-    const int cw = warp - 2, l16 = lane & 15, hi = lane >> 4;
-    const unsigned int row0 = cw * 8 + hi, box = (l16 >> 3) * 8192u;
-    int u_l = blockIdx.x, c_l = 0, c1_l = 0, g_l = 0;  // cursor of the exponents
-    auto locate = [&]() {
-      if (u_l >= a.units) return;
-      int tile;
-      dw_unit(a, u_l, tile, c_l, c1_l);
-      g_l = tile % a.i_tiles * (kTileI / kCkGroup) + (lane & 3);
-    };
-    auto next_exp = [&]() -> unsigned int {
-      unsigned int e = kCkMinExp;
-      if (u_l < a.units) {
-        const long long t = (long long)c_l * kChunk + cw * 8 + (lane >> 2);
-        if (t < a.rows && g_l < a.groups) e = __ldg(a.exps + t * a.groups + g_l);
-        if (++c_l == c1_l) {
-          u_l += gridDim.x;
-          locate();
-        }
-      }
-      return e;
-    };
-    locate();
-    unsigned int e0 = next_exp(), e1 = next_exp();
-    int s = 0;
-    unsigned int ph = 0;
+    // ---- MMAs: the warp walks through the chunks, one elected lane issues ----
+    // fp32 accumulator, bfloat16 factors, both MN-major, M = 128; N is set per tile
+    const unsigned int idesc0 = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | (8u << 24);
+    const unsigned long long dx0 = pw_smem_desc(base, 8192, 1024, 2), dd0 = pw_smem_desc(base + kXBytes, 8192, 1024, 2);
+    int s = 0, b = 0;
+    unsigned int ph = 0, aph = 0;
     bool ok = true;
     for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
       int tile, c0, c1;
       dw_unit(a, u, tile, c0, c1);
-      const int o = tile / a.i_tiles * BN + l16 * 8;
-#pragma unroll 1
+      const int o0 = tile / a.i_tiles * BN;
+      const int n = min(BN, (a.c_out - o0 + 15) & ~15);
+      const unsigned int idesc = idesc0 | ((unsigned)(n >> 3) << 17);
+      int run = 0;
       for (int c = c0; c < c1; ++c) {
-        const unsigned int e2 = next_exp();
-        if (!pw_wait(&full[s], ph) || *abort_v) { ok = false; break; }
-        unsigned char *st = sm + s * STAGE;
+        // dy and the codes of the stage have landed when its converters have arrived: they waited for them
+        if ((run == 0 && !pw_wait(&acc_empty[b], aph ^ 1u)) || !pw_wait(&conv[s], ph) || *abort_v) { ok = false; break; }
+        tc_fence_after();
+        const bool last = c == c1 - 1 || (KEEP32 && run == RUN - 1);
+        const unsigned long long so = (unsigned long long)(s * STAGE) >> 4;
+        const unsigned int d = tmem_base + b * BN;
+        const int steps = (int)min((long long)kChunk / 16, (a.rows - (long long)c * kChunk + 15) / 16);
+        if (elect_one()) {
+          // the small parts first: a sum that only grows loses least
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const unsigned int r = row0 + 2 * p;
-          const uint2 code = *reinterpret_cast<const uint2 *>(st + CODES + r * kTileI + l16 * 8);
-          const unsigned int e = __shfl_sync(0xffffffffu, e0, (2 * p + hi) * 4 + (l16 >> 2));
-          *reinterpret_cast<uint4 *>(st + box + r * 128 + (((l16 & 7) ^ (2 * p + hi)) << 4)) = dw_expand(code, e);
+          for (int p = PARTS - 1; p >= 0; --p) {
+            const unsigned long long dx = dx0 + so, dd = dd0 + so + (unsigned)(p * (DYB >> 4));
+#pragma unroll
+            for (int j = 0; j < kChunk / 16; ++j)  // a step is 16 rows of 128 bytes
+              if (j < steps) tc_mma_f16(d, dx + j * 128, dd + j * 128, idesc, run || j || p < PARTS - 1 ? 1u : 0u);
+          }
+          tc_commit(&empty[s]);
+          if (last) tc_commit(&acc_full[b]);
         }
-        if (DY != DY_TMA) {
+        __syncwarp();
+        ++run;
+        if (last) {
+          run = 0;
+          if (++b == NACC) { b = 0; aph ^= 1u; }
+        }
+        if (++s == STAGES) { s = 0; ph ^= 1u; }
+      }
+    }
+    if (!ok) {
+      if (lane == 0 && !*abort_v) { atomicExch(a.flag, 1); *abort_v = 1; }
+      if (elect_one()) tc_commit(drained);  // the MMAs in flight end before the tensor memory is given back
+      __syncwarp();
+      pw_wait(drained, 0);
+    }
+  } else if (warp < kFirstEpi) {
+    // ---- converters: group g has the chunks n = g, g + STAGES, ... of this CTA and with them stage g; a warp has TOKENS tokens
+    // of the chunk, a pass is two tokens, a lane eight channels. The exponents of a warp's tokens come by byte loads, one chunk
+    // of the group ahead. The code is kept short: unrolled over several chunks it threw the instructions of the warps that
+    // issue the loads and the MMAs out of the instruction cache ----
+    const int g = (warp - 2) / GROUP, l16 = lane & 15, hi = lane >> 4;
+    const unsigned int tok0 = ((warp - 2) % GROUP) * TOKENS, box = (l16 >> 3) * 8192u;
+    unsigned char *st = sm + g * STAGE;
+    constexpr int EX = TOKENS * 4 / 32;  // exponents per lane: four groups of 32 channels per token
+    int u = blockIdx.x, tile = 0, c = 0, c1 = 0;
+    // the cursor moves `by` chunks on, into the next units where need be
+    auto move = [&](int by) {
+      c += by;
+      while (u < a.units && c >= c1) {
+        int c0;
+        const int over = c - c1;
+        u += gridDim.x;
+        if (u < a.units) {
+          dw_unit(a, u, tile, c0, c1);
+          c = c0 + over;
+        }
+      }
+    };
+    auto exponents = [&](unsigned int(&e)[EX]) {
+      const int gr = tile % a.i_tiles * (kTileI / kCkGroup) + (lane & 3);
+#pragma unroll
+      for (int k = 0; k < EX; ++k) {
+        const long long t = (long long)c * kChunk + tok0 + k * 8 + (lane >> 2);
+        e[k] = u < a.units && t < a.rows && gr < a.groups ? __ldg(a.exps + t * a.groups + gr) : kCkMinExp;
+      }
+    };
+    unsigned int ex[EX], ex_next[EX], ph = 0;
+    if (u < a.units) dw_unit(a, u, tile, c, c1);
+    move(g);
+    exponents(ex);
+    bool ok = true;
+    while (u < a.units) {
+      const int c_now = c, o = tile / a.i_tiles * BN + l16 * 8;
+      move(STAGES);
+      exponents(ex_next);
+      if (!pw_wait(&full[g], ph) || *abort_v) { ok = false; break; }
+#pragma unroll
+      for (int p = 0; p < TOKENS / 2; ++p) {
+        const unsigned int r = tok0 + 2 * p + hi;
+        const uint2 code = *reinterpret_cast<const uint2 *>(st + S::CODES + r * kTileI + l16 * 8);
+        const unsigned int e = __shfl_sync(0xffffffffu, ex[p / 4], (2 * (p & 3) + hi) * 4 + (l16 >> 2));
+        *reinterpret_cast<uint4 *>(st + box + r * 128 + (((l16 & 7) ^ (r & 7)) << 4)) = dw_expand(code, e);
+      }
+      if (DY != DY_TMA) {
 #pragma unroll 1
-          for (int p = 0; p < 4; ++p) {
-            const unsigned int r = row0 + 2 * p;
-            const long long t = (long long)c * kChunk + r;
-            DyVec<T> x;
-            if (DY == DY_RAW) x.load_shared(st + RAW, r, l16);
-            else x.load(static_cast<const T *>(a.dy) + t * a.ld, o, t < a.rows ? a.c_out : 0);
-            float v[8];
-            x.get(v);
-            unsigned char *to = st + kXBytes + box + r * 128 + (((l16 & 7) ^ (2 * p + hi)) << 4);
+        for (int p = 0; p < TOKENS / 2; ++p) {
+          const unsigned int r = tok0 + 2 * p + hi;
+          const long long t = (long long)c_now * kChunk + r;
+          DyVec<T> x;
+          if (DY == DY_RAW) x.load_shared(st + S::RAW, r, l16);
+          else x.load(static_cast<const T *>(a.dy) + t * a.ld, o, t < a.rows ? a.c_out : 0);
+          float v[8];
+          x.get(v);
+          unsigned char *to = st + kXBytes + box + r * 128 + (((l16 & 7) ^ (r & 7)) << 4);
 #pragma unroll
-            for (int q = 0; q < PARTS; ++q) {
-              unsigned int w[4];
+          for (int q = 0; q < PARTS; ++q) {
+            unsigned int w[4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const unsigned int lo = dw_head(v[2 * j]), up = dw_head(v[2 * j + 1]);
-                w[j] = (lo >> 16) | up;
-              }
-              *reinterpret_cast<uint4 *>(to + q * DYB) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int j = 0; j < 4; ++j) {
+              const unsigned int lo = dw_head(v[2 * j]), up = dw_head(v[2 * j + 1]);
+              w[j] = (lo >> 16) | up;
             }
+            *reinterpret_cast<uint4 *>(to + q * DYB) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // visible to the tensor core's reads
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&conv[s]);
-        e0 = e1;
-        e1 = e2;
-        if (++s == a.stages) { s = 0; ph ^= 1u; }
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // visible to the tensor core's reads
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&conv[g]);
+#pragma unroll
+      for (int k = 0; k < EX; ++k) ex[k] = ex_next[k];
+      ph ^= 1u;
     }
     if (!ok && lane == 0 && !*abort_v) { atomicExch(a.flag, 1); *abort_v = 1; }
   } else {
@@ -356,42 +362,49 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
       TW *dw = static_cast<TW *>(a.dw) + (long long)o0 * a.c_in + i;
       float *part = whole ? nullptr : a.parts + ((long long)(u - a.full) * BN + half * HALF) * kTileI + il;
       const bool i_ok = i < a.c_in;
-      auto store = [&](int col, float v) {
-        if (col >= n) return;
-        if (!whole) {
-          part[col * kTileI] = v;
-        } else if (i_ok) {
-          TW *q = dw + (long long)col * a.c_in;
-          *q = Elem<TW>::from_f32(a.accum ? __fadd_rn(Elem<TW>::to_f32(*q), v) : v);
-        }
+      // Run r of the unit: the first is stored (or added to what is there, where the caller accumulates), the others are added.
+      // The sixteen loads go out together, before any of the sums is stored.
+      auto add_to = [&](auto *to, long long stride, int q, float *v) {
+        using E = std::remove_pointer_t<decltype(to)>;
+        E old[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) old[j] = q + j < n ? to[(q + j) * stride] : Elem<E>::from_f32(0.0f);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = __fadd_rn(Elem<E>::to_f32(old[j]), v[j]);
       };
-      const int runs = KEEP32 ? (c1 - c0 + kRun - 1) / kRun : 1;
-      float sum[KEEP32 ? HALF : 1];
+      auto put = [&](auto *to, long long stride, int q, const float *v) {
+        using E = std::remove_pointer_t<decltype(to)>;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (q + j < n) to[(q + j) * stride] = Elem<E>::from_f32(v[j]);
+      };
+      const int runs = KEEP32 ? (c1 - c0 + RUN - 1) / RUN : 1;
       for (int r = 0; ok && r < runs; ++r) {
         if (!pw_wait(&acc_full[b], aph) || *abort_v) { ok = false; break; }
         tc_fence_after();
         const unsigned int taddr = tmem_base + ((unsigned)(quarter * 32) << 16) + b * BN + half * HALF;
+#pragma unroll 1
+        for (int q = 0; q < HALF && q < n; q += 16) {
+          unsigned int acc[2][8];
+          tc_ld8(taddr + q, acc[0]);
+          tc_ld8(taddr + q + 8, acc[1]);
+          tc_ld_wait8(acc[0]);
+          tc_ld_wait8(acc[1]);
+          float v[16];
 #pragma unroll
-        for (int q = 0; q < HALF; q += 8) {
-          if (!KEEP32 && q >= n) break;
-          unsigned int acc[8];
-          tc_ld8(taddr + q, acc);
-          tc_ld_wait8(acc);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float v = __uint_as_float(acc[j]);
-            if (KEEP32) sum[q + j] = r ? __fadd_rn(sum[q + j], v) : v;
-            else store(q + j, v);
+          for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(acc[j >> 3][j & 7]);
+          if (!whole) {
+            if (r) add_to(part, kTileI, q, v);
+            put(part, kTileI, q, v);
+          } else if (i_ok) {
+            if (r || a.accum) add_to(dw, a.c_in, q, v);
+            put(dw, a.c_in, q, v);
           }
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&acc_empty[b]);
         if (++b == NACC) { b = 0; aph ^= 1u; }
-      }
-      if (KEEP32 && ok) {
-#pragma unroll
-        for (int q = 0; q < HALF; ++q) store(q, sum[q]);
       }
     }
     if (!ok && lane == 0 && !*abort_v) { atomicExch(a.flag, 1); *abort_v = 1; }
@@ -489,7 +502,7 @@ DwPlan dw_plan(const dwbnq_affine_desc &d, bool wide) {
   p.bytes = 256 + p.parts_bytes + up256((size_t)kDbSlices * d.c_out * 4);
   return p;
 }
-bool dw_wide(const dwbnq_affine_desc &d) { return d.dtype == DWBNQ_BF16 && d.dw_dtype == DWBNQ_BF16; }
+bool dw_wide(const dwbnq_affine_desc &d) { return d.dtype == DWBNQ_BF16; }
 
 typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -508,13 +521,11 @@ EncodeFn encode_fn() {
   return fn;
 }
 
-template <typename T, typename TW, int PARTS, int DY, int BN, bool KEEP32>
-int launch_dw(const CUtensorMap &tm, const CUtensorMap &tc, DwArgs &a, cudaStream_t stream) {
-  constexpr int STAGE = DwStage<PARTS, BN, DY == DY_RAW, (int)sizeof(T)>::BYTES;
-  constexpr int fit = (kSmemMax - 2048) / STAGE;
-  a.stages = fit < kMaxStages ? fit : kMaxStages;
-  const int smem = a.stages * STAGE + 1024;
-  auto kern = affine_dw_kernel<T, TW, PARTS, DY, BN, KEEP32>;
+template <typename T, typename TW, int PARTS, int DY, int BN>
+int launch_dw(const CUtensorMap &tm, const CUtensorMap &tc, const DwArgs &a, cudaStream_t stream) {
+  using S = DwStage<PARTS, BN, DY, (int)sizeof(T)>;
+  const int smem = S::COUNT * S::BYTES + 1024;
+  auto kern = affine_dw_kernel<T, TW, PARTS, DY, BN>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return fail_cuda(e, "affine_dw_kernel attributes");
   const int sms = sm_count(-1);
@@ -572,17 +583,17 @@ int run_t(const dwbnq_affine_desc &d, const void *codes, const void *exps, const
     }
     if constexpr (sizeof(TW) == 4) {
       if (d.dtype == DWBNQ_F32)
-        st = tma ? launch_dw<float, TW, 3, DY_RAW, 128, true>(tm, tc, a, stream) : launch_dw<float, TW, 3, DY_LOAD, 128, true>(tm, tc, a, stream);
+        st = tma ? launch_dw<float, TW, 3, DY_RAW, 128>(tm, tc, a, stream) : launch_dw<float, TW, 3, DY_LOAD, 128>(tm, tc, a, stream);
       else if (d.dtype == DWBNQ_F16)
-        st = tma ? launch_dw<__half, TW, 2, DY_RAW, 128, true>(tm, tc, a, stream) : launch_dw<__half, TW, 2, DY_LOAD, 128, true>(tm, tc, a, stream);
+        st = tma ? launch_dw<__half, TW, 2, DY_RAW, 128>(tm, tc, a, stream) : launch_dw<__half, TW, 2, DY_LOAD, 128>(tm, tc, a, stream);
       else
-        st = tma ? launch_dw<__nv_bfloat16, TW, 1, DY_TMA, 128, true>(tm, tc, a, stream)
-                 : launch_dw<__nv_bfloat16, TW, 1, DY_LOAD, 128, true>(tm, tc, a, stream);
+        st = tma ? launch_dw<__nv_bfloat16, TW, 1, DY_TMA, 256>(tm, tc, a, stream)
+                 : launch_dw<__nv_bfloat16, TW, 1, DY_LOAD, 128>(tm, tc, a, stream);
     } else if constexpr (std::is_same<TW, __half>::value) {
-      st = tma ? launch_dw<__half, TW, 2, DY_RAW, 128, true>(tm, tc, a, stream) : launch_dw<__half, TW, 2, DY_LOAD, 128, true>(tm, tc, a, stream);
+      st = tma ? launch_dw<__half, TW, 2, DY_RAW, 128>(tm, tc, a, stream) : launch_dw<__half, TW, 2, DY_LOAD, 128>(tm, tc, a, stream);
     } else {
-      st = tma ? launch_dw<__nv_bfloat16, TW, 1, DY_TMA, 256, false>(tm, tc, a, stream)
-               : launch_dw<__nv_bfloat16, TW, 1, DY_LOAD, 128, true>(tm, tc, a, stream);
+      st = tma ? launch_dw<__nv_bfloat16, TW, 1, DY_TMA, 256>(tm, tc, a, stream)
+               : launch_dw<__nv_bfloat16, TW, 1, DY_LOAD, 128>(tm, tc, a, stream);
     }
     if (st != DWBNQ_OK) return st;
     if (p.segs > 1) {

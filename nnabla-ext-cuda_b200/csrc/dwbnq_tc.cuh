@@ -48,6 +48,14 @@ __device__ __forceinline__ bool pw_wait(unsigned long long *bar, unsigned int pa
   }
   return ok;
 }
+// True in one lane of a converged warp. TMA and tcgen05 instructions take their operands from uniform registers: issued under this
+// predicate from code the whole warp walks through, addresses and descriptors stay there; issued under `lane == 0` every
+// operand is moved over one instruction at a time (the MMA thread of the weight gradient: 1400 cycles per four MMAs against 600).
+__device__ __forceinline__ bool elect_one() {
+  unsigned int ok;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok));
+  return ok != 0;
+}
 __device__ __forceinline__ void mbar_arrive(unsigned long long *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
