@@ -29,11 +29,9 @@ namespace dwbnq {
 
 namespace {
 
-constexpr int kChunk = 64;        // tokens per pipeline stage
 constexpr int kTileI = 128;       // input channels per tile = TMEM lanes
 constexpr int kConvWarps = 16, kFirstEpi = 2 + kConvWarps, kEpiWarps = 8;
 constexpr int kThreads = 32 * (kFirstEpi + kEpiWarps);
-constexpr int kXBytes = kChunk * kTileI * 2;
 constexpr int kMaxStages = 4, kTmemCols = 512, kMaxAcc = 4;
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kPlanSms = 148;     // SMs of a B200: the cut of the last wave does not depend on the device it is asked on
@@ -45,7 +43,7 @@ struct DwArgs {
   long long ld, rows;
   int c_in, c_out, groups;
   int i_tiles;
-  int chunks;              // ceil(rows / 64)
+  int chunks;              // ceil(rows / tokens per chunk)
   int full, segs, units;   // units 0 .. full-1: whole tiles; then segs parts of every further tile
   void *dw;
   float *parts;            // [unit - full][tile columns][128]
@@ -86,18 +84,47 @@ __device__ __forceinline__ uint4 dw_expand(uint2 c, unsigned int b) {
   return r;
 }
 
-// The leading bfloat16 of v (truncated) and what is left, exactly; an infinity leaves 0, a NaN stays one.
-__device__ __forceinline__ unsigned int dw_head(float &v) {
-  unsigned int h = __float_as_uint(v) & 0xffff0000u;
-  if ((__float_as_uint(v) & 0x7fffffffu) > 0x7f800000u) h = 0x7fc00000u;
-  v = (h & 0x7f800000u) == 0x7f800000u ? 0.0f : __fsub_rn(v, __uint_as_float(h));
-  return h;
+// Eight values as PARTS vectors of eight bfloat16 that add up to them exactly: the truncated head of what is left (the upper half
+// of the word, taken by the byte permutation that packs it), then the rest. A NaN stays one through every part; an infinity's rest
+// would be one too, so a vector that holds a value that is not finite takes the second way.
+template <int PARTS>
+__device__ __forceinline__ void dw_split(float *v, uint4 *part) {
+  unsigned int top = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+  if (PARTS > 1 && top >= 0x7f800000u) {
+    const float inf = __uint_as_float(0x7f800000u);
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) {
+      unsigned int w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        w[j] = v[j] != v[j] ? 0x7fc0u : __float_as_uint(v[j]) >> 16;
+        v[j] = fabsf(v[j]) < inf ? __fsub_rn(v[j], __uint_as_float(w[j] << 16)) : 0.0f;
+      }
+      part[q] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+    }
+    return;
+  }
+#pragma unroll
+  for (int q = 0; q < PARTS; ++q) {
+    unsigned int w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = __byte_perm(__float_as_uint(v[2 * j]), __float_as_uint(v[2 * j + 1]), 0x7632);
+    part[q] = make_uint4(w[0], w[1], w[2], w[3]);
+    if (q + 1 < PARTS)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __fsub_rn(v[j], __uint_as_float(__float_as_uint(v[j]) & 0xffff0000u));
+  }
 }
 
 // How dy reaches the tensor cores: by TMA as it is (bfloat16); by TMA into a buffer from which the converters split it (float16,
 // float32); or loaded and split by the converters (rows that are not multiples of 16 bytes, which TMA cannot take).
 enum DyMode : int { DY_TMA = 0, DY_RAW = 1, DY_LOAD = 2 };
-template <typename T> struct DyBox { static constexpr int COLS = 128 / (int)sizeof(T); };  // a box is 64 tokens x 128 bytes
+template <typename T> struct DyBox { static constexpr int COLS = 128 / (int)sizeof(T); };  // a box is a chunk's tokens x 128 bytes
+// Tokens per pipeline stage: where dy is split a stage also holds it as it came and in parts, and four stages of 32 tokens
+// cover the loads' latency better than two of 64.
+__host__ __device__ constexpr int dw_chunk(int dy_mode) { return dy_mode == DY_TMA ? 64 : 32; }
 
 // Eight consecutive elements of a row of dy.
 template <typename T> struct DyVec {
@@ -105,7 +132,7 @@ template <typename T> struct DyVec {
   // elements 8 i .. 8 i + 7 of row r of the boxes at `raw`; zero beyond the tensor, as TMA filled them
   __device__ __forceinline__ void load_shared(const unsigned char *raw, unsigned int r, int i) {
     constexpr int PER = DyBox<T>::COLS / 8;  // vectors per box row
-    const uint4 *p = reinterpret_cast<const uint4 *>(raw + (i / PER) * 8192 + r * 128 + (i % PER) * 8 * sizeof(T));
+    const uint4 *p = reinterpret_cast<const uint4 *>(raw + (i / PER) * (dw_chunk(DY_RAW) * 128) + r * 128 + (i % PER) * 8 * sizeof(T));
 #pragma unroll
     for (int k = 0; k < 8 * (int)sizeof(T) / 16; ++k) w[k] = p[k];
   }
@@ -128,8 +155,8 @@ template <typename T> struct DyVec {
 // converters' groups are as many, so that each stage's barriers are always awaited by the same group (a parity wait cannot
 // tell a phase from the one after the next).
 template <int PARTS, int BN, int DY, int TBYTES> struct DwStage {
-  static constexpr int DYB = kChunk * BN * 2, CODES = kXBytes + PARTS * DYB, RAW = CODES + kChunk * kTileI,
-                       BYTES = RAW + (DY == DY_RAW ? kChunk * BN * TBYTES : 0), COUNT = 4 * BYTES + 2048 <= kSmemMax ? 4 : 2;
+  static constexpr int CHUNK = dw_chunk(DY), XB = CHUNK * kTileI * 2, DYB = CHUNK * BN * 2, CODES = XB + PARTS * DYB,
+                       RAW = CODES + CHUNK * kTileI, BYTES = RAW + (DY == DY_RAW ? CHUNK * BN * TBYTES : 0), COUNT = 4 * BYTES + 2048 <= kSmemMax ? 4 : 2;
 };
 
 // T: type of dy; TW: type of dw (32 bits: sums in short runs); PARTS: bfloat16 parts of dy; BN: output channels per tile.
@@ -137,10 +164,11 @@ template <typename T, typename TW, int PARTS, int DY, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
 affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ CUtensorMap tm_codes, const DwArgs a) {
   using S = DwStage<PARTS, BN, DY, (int)sizeof(T)>;
-  constexpr int DYB = S::DYB, STAGE = S::BYTES, STAGES = S::COUNT;
-  constexpr int GROUP = kConvWarps / STAGES, TOKENS = kChunk / GROUP;  // converter warps per group, tokens per warp and chunk
+  constexpr int CHUNK = S::CHUNK, XB = S::XB, DYB = S::DYB, STAGE = S::BYTES, STAGES = S::COUNT;
+  constexpr int BOX = CHUNK * 128;                    // bytes of a box of CHUNK tokens
+  constexpr int GROUP = kConvWarps / STAGES, TOKENS = CHUNK / GROUP;  // converter warps per group, tokens per warp and chunk
   constexpr bool KEEP32 = sizeof(TW) == 4;
-  constexpr int RUN = PARTS == 1 ? 16 : PARTS == 2 ? 8 : 4;  // chunks per run: the more digits in dy, the more the adder drops
+  constexpr int RUN = (PARTS == 1 ? 1024 : PARTS == 2 ? 512 : 256) / CHUNK;  // chunks per run: the more digits in dy, the more the adder drops
   constexpr int NACC = kTmemCols / BN < kMaxAcc ? kTmemCols / BN : kMaxAcc;
   constexpr int HALF = BN / 2;                        // columns per epilogue warp
   static_assert(DY != DY_TMA || PARTS == 1, "dy as it is has one part");
@@ -185,7 +213,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
   volatile int *abort_v = &abort_s;
 
   if (warp == 0) {
-    // ---- TMA loads: the codes and, where it can take them, dy: boxes of 64 tokens x 128 bytes, zero beyond the tensors ----
+    // ---- TMA loads: the codes and, where it can take them, dy: boxes of a chunk's tokens x 128 bytes, zero beyond the tensors ----
     int s = 0, issued = 0;
     unsigned int ph = 0;
     bool ok = true;
@@ -193,17 +221,17 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
       int tile, c0, c1;
       dw_unit(a, u, tile, c0, c1);
       const int ot = tile / a.i_tiles, o0 = ot * BN, i0 = (tile - ot * a.i_tiles) * kTileI;
-      constexpr int COLS = DyBox<T>::COLS, MAXBOX = BN / COLS, DYAT = DY == DY_RAW ? S::RAW : kXBytes;
+      constexpr int COLS = DyBox<T>::COLS, MAXBOX = BN / COLS, DYAT = DY == DY_RAW ? S::RAW : XB;
       const int boxes = DY == DY_LOAD ? 0 : min(MAXBOX, (a.c_out - o0 + COLS - 1) / COLS);
       for (int c = c0; c < c1; ++c) {
         if (!pw_wait(&empty[s], ph ^ 1u) || *abort_v) { ok = false; break; }
         if (elect_one()) {
           unsigned char *st = sm + s * STAGE;
-          mbar_expect_tx(&full[s], (boxes + 1) * 8192);
-          tma_load_2d(st + S::CODES, &tm_codes, i0, c * kChunk, &full[s]);
+          mbar_expect_tx(&full[s], (boxes + 1) * BOX);
+          tma_load_2d(st + S::CODES, &tm_codes, i0, c * CHUNK, &full[s]);
 #pragma unroll
           for (int q = 0; q < MAXBOX; ++q)
-            if (q < boxes) tma_load_2d(st + DYAT + q * 8192, &tm_dy, o0 + q * COLS, c * kChunk, &full[s]);
+            if (q < boxes) tma_load_2d(st + DYAT + q * BOX, &tm_dy, o0 + q * COLS, c * CHUNK, &full[s]);
         }
         __syncwarp();
         if (issued < STAGES) ++issued;
@@ -222,7 +250,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
     // ---- MMAs: the warp walks through the chunks, one elected lane issues ----
     // fp32 accumulator, bfloat16 factors, both MN-major, M = 128; N is set per tile
     const unsigned int idesc0 = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | (8u << 24);
-    const unsigned long long dx0 = pw_smem_desc(base, 8192, 1024, 2), dd0 = pw_smem_desc(base + kXBytes, 8192, 1024, 2);
+    const unsigned long long dx0 = pw_smem_desc(base, BOX, 1024, 2), dd0 = pw_smem_desc(base + XB, BOX, 1024, 2);
     int s = 0, b = 0;
     unsigned int ph = 0, aph = 0;
     bool ok = true;
@@ -240,14 +268,14 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
         const bool last = c == c1 - 1 || (KEEP32 && run == RUN - 1);
         const unsigned long long so = (unsigned long long)(s * STAGE) >> 4;
         const unsigned int d = tmem_base + b * BN;
-        const int steps = (int)min((long long)kChunk / 16, (a.rows - (long long)c * kChunk + 15) / 16);
+        const int steps = (int)min((long long)CHUNK / 16, (a.rows - (long long)c * CHUNK + 15) / 16);
         if (elect_one()) {
           // the small parts first: a sum that only grows loses least
 #pragma unroll
           for (int p = PARTS - 1; p >= 0; --p) {
             const unsigned long long dx = dx0 + so, dd = dd0 + so + (unsigned)(p * (DYB >> 4));
 #pragma unroll
-            for (int j = 0; j < kChunk / 16; ++j)  // a step is 16 rows of 128 bytes
+            for (int j = 0; j < CHUNK / 16; ++j)  // a step is 16 rows of 128 bytes
               if (j < steps) tc_mma_f16(d, dx + j * 128, dd + j * 128, idesc, run || j || p < PARTS - 1 ? 1u : 0u);
           }
           tc_commit(&empty[s]);
@@ -274,8 +302,9 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
     // of the group ahead. The code is kept short: unrolled over several chunks it threw the instructions of the warps that
     // issue the loads and the MMAs out of the instruction cache ----
     const int g = (warp - 2) / GROUP, l16 = lane & 15, hi = lane >> 4;
-    const unsigned int tok0 = ((warp - 2) % GROUP) * TOKENS, box = (l16 >> 3) * 8192u;
+    const unsigned int tok0 = ((warp - 2) % GROUP) * TOKENS, box = (l16 >> 3) * (unsigned)BOX;
     unsigned char *st = sm + g * STAGE;
+    static_assert(TOKENS >= 8, "a byte of exponents for every lane");
     constexpr int EX = TOKENS * 4 / 32;  // exponents per lane: four groups of 32 channels per token
     int u = blockIdx.x, tile = 0, c = 0, c1 = 0;
     // the cursor moves `by` chunks on, into the next units where need be
@@ -295,7 +324,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
       const int gr = tile % a.i_tiles * (kTileI / kCkGroup) + (lane & 3);
 #pragma unroll
       for (int k = 0; k < EX; ++k) {
-        const long long t = (long long)c * kChunk + tok0 + k * 8 + (lane >> 2);
+        const long long t = (long long)c * CHUNK + tok0 + k * 8 + (lane >> 2);
         e[k] = u < a.units && t < a.rows && gr < a.groups ? __ldg(a.exps + t * a.groups + gr) : kCkMinExp;
       }
     };
@@ -320,23 +349,17 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
 #pragma unroll 1
         for (int p = 0; p < TOKENS / 2; ++p) {
           const unsigned int r = tok0 + 2 * p + hi;
-          const long long t = (long long)c_now * kChunk + r;
+          const long long t = (long long)c_now * CHUNK + r;
           DyVec<T> x;
           if (DY == DY_RAW) x.load_shared(st + S::RAW, r, l16);
           else x.load(static_cast<const T *>(a.dy) + t * a.ld, o, t < a.rows ? a.c_out : 0);
           float v[8];
           x.get(v);
-          unsigned char *to = st + kXBytes + box + r * 128 + (((l16 & 7) ^ (r & 7)) << 4);
+          unsigned char *to = st + XB + box + r * 128 + (((l16 & 7) ^ (r & 7)) << 4);
+          uint4 part[PARTS];
+          dw_split<PARTS>(v, part);
 #pragma unroll
-          for (int q = 0; q < PARTS; ++q) {
-            unsigned int w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const unsigned int lo = dw_head(v[2 * j]), up = dw_head(v[2 * j + 1]);
-              w[j] = (lo >> 16) | up;
-            }
-            *reinterpret_cast<uint4 *>(to + q * DYB) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+          for (int q = 0; q < PARTS; ++q) *reinterpret_cast<uint4 *>(to + q * DYB) = part[q];
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // visible to the tensor core's reads
@@ -479,14 +502,15 @@ struct DwPlan {
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // `wide`: tiles of 256 output channels. Whole waves of kPlanSms tiles are walked uncut; the R tiles left over are cut into
-// the number of parts that costs least, in chunks of 64 tokens on the busiest SM: ceil(R s / SMs) parts of ceil(chunks / s)
+// the number of parts that costs least, in chunks on the busiest SM: ceil(R s / SMs) parts of ceil(chunks / s)
 // chunks, each with about 4 chunks' worth of read-back, and 16 for the second kernel and the parts' traffic.
 DwPlan dw_plan(const dwbnq_affine_desc &d, bool wide) {
+  const int chunk = dw_chunk(wide ? DY_TMA : DY_LOAD);
   DwPlan p;
   p.bn = wide ? 256 : 128;
   p.i_tiles = (d.c_in + kTileI - 1) / kTileI;
   p.o_tiles = (d.c_out + p.bn - 1) / p.bn;
-  p.chunks = (int)((d.rows + kChunk - 1) / kChunk);
+  p.chunks = (int)((d.rows + chunk - 1) / chunk);
   const long long tiles = (long long)p.i_tiles * p.o_tiles;
   const int rest = (int)(tiles % kPlanSms);
   p.full = (int)(tiles - rest);
@@ -564,16 +588,16 @@ int run_t(const dwbnq_affine_desc &d, const void *codes, const void *exps, const
     std::memset(&tm, 0, sizeof(tm));
     std::memset(&tc, 0, sizeof(tc));
     if (!encode_fn()) return fail(DWBNQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-    const cuuint32_t es[2] = {1, 1};
+    const cuuint32_t es[2] = {1, 1}, chunk = (cuuint32_t)dw_chunk(d.dtype == DWBNQ_BF16 && tma ? DY_TMA : tma ? DY_RAW : DY_LOAD);
     const cuuint64_t cdim[2] = {(cuuint64_t)a.groups * kCkGroup, (cuuint64_t)d.rows}, cstr[1] = {cdim[0]};
-    const cuuint32_t cbox[2] = {kTileI, kChunk};
+    const cuuint32_t cbox[2] = {kTileI, chunk};
     CUresult r = encode_fn()(&tc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(codes), cdim, cstr, cbox, es,
                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(DWBNQ_ERR_CUDA, "cuTensorMapEncodeTiled(codes) failed with CUresult %d", (int)r);
     if (tma) {
       const cuuint64_t dim[2] = {(cuuint64_t)d.c_out, (cuuint64_t)d.rows}, str[1] = {(cuuint64_t)d.ld_dy * eb};
-      const cuuint32_t box[2] = {(cuuint32_t)(128 / eb), kChunk};
+      const cuuint32_t box[2] = {(cuuint32_t)(128 / eb), chunk};
       const bool as_is = d.dtype == DWBNQ_BF16;
       r = encode_fn()(&tm, as_is ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : eb == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
                       2, const_cast<void *>(dy), dim, str, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
