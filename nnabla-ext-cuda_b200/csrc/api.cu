@@ -914,7 +914,7 @@ int dwbnq_w4_affine_fwd(const dwbnq_w4_desc *desc, int64_t rows, int64_t ld_x, c
   st = enter_device(device, &dev);
   if (st != DWBNQ_OK) return st;
   if (rows == 0 || desc->c_out == 0) return DWBNQ_OK;
-  return launch_w4_affine(*desc, rows, ld_x, x, packed, b, ld_y, y, static_cast<cudaStream_t>(stream));
+  return launch_w4_affine(*desc, rows, ld_x, x, packed, b, ld_y, y, dev, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -173,7 +173,7 @@ int launch_w4_quantize(int dtype, int c_out, int c_in, int group, long long ld, 
 int launch_w4_pack(const dwbnq_w4_desc &d, const void *codes, const void *scales, const void *zeros, void *packed,
                    cudaStream_t stream);
 int launch_w4_affine(const dwbnq_w4_desc &d, long long rows, long long ld_x, const void *x, const void *packed, const void *b,
-                     long long ld_y, void *y, cudaStream_t stream);
+                     long long ld_y, void *y, int dev, cudaStream_t stream);
 
 // ---- communicator (comm.cpp) --------------------------------------------------------------
 int comm_allreduce_max(void *comm, float *buf, long long count, cudaStream_t stream,
