@@ -67,20 +67,20 @@ __device__ __forceinline__ void dw_unit(const DwArgs &a, int u, int &tile, int &
 
 // Eight codes (two words) as bfloat16 values of step `step2` (the step twice): k = (128 + low seven bits) - (128 or
 // 256 for the sign bit), both exact in bfloat16, then the exact product with a power of two.
-__device__ __forceinline__ unsigned int dw_pair(unsigned int two, __nv_bfloat162 step2) {
-  const unsigned int lo = (two & 0x007f007fu) | 0x43004300u, hi = (two & 0x00800080u) | 0x43004300u;
+__device__ __forceinline__ unsigned int dw_pair(unsigned int two, __nv_bfloat162 step2, unsigned int magic) {  // magic: 128, twice
+  const unsigned int lo = and_or(two, 0x007f007fu, magic), hi = and_or(two, 0x00800080u, magic);
   const __nv_bfloat162 k = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&lo), *reinterpret_cast<const __nv_bfloat162 *>(&hi));
   const __nv_bfloat162 v = __hmul2(k, step2);
   return *reinterpret_cast<const unsigned int *>(&v);
 }
-__device__ __forceinline__ uint4 dw_expand(uint2 c, unsigned int b) {
+__device__ __forceinline__ uint4 dw_expand(uint2 c, unsigned int b, unsigned int magic) {
   const unsigned int s = b == kCkNonFinite ? 0x7fc07fc0u : b * 0x00800080u - 0x03000300u;  // (b - 6) << 7, twice
   const __nv_bfloat162 s2 = *reinterpret_cast<const __nv_bfloat162 *>(&s);
   uint4 r;
-  r.x = dw_pair(__byte_perm(c.x, 0u, 0x4140), s2);
-  r.y = dw_pair(__byte_perm(c.x, 0u, 0x4342), s2);
-  r.z = dw_pair(__byte_perm(c.y, 0u, 0x4140), s2);
-  r.w = dw_pair(__byte_perm(c.y, 0u, 0x4342), s2);
+  r.x = dw_pair(__byte_perm(c.x, 0u, 0x4140), s2, magic);
+  r.y = dw_pair(__byte_perm(c.x, 0u, 0x4342), s2, magic);
+  r.z = dw_pair(__byte_perm(c.y, 0u, 0x4140), s2, magic);
+  r.w = dw_pair(__byte_perm(c.y, 0u, 0x4342), s2, magic);
   return r;
 }
 
@@ -328,6 +328,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
         e[k] = u < a.units && t < a.rows && gr < a.groups ? __ldg(a.exps + t * a.groups + gr) : kCkMinExp;
       }
     };
+    const unsigned int magic = opaque_constant(0x43004300u);
     unsigned int ex[EX], ex_next[EX], ph = 0;
     if (u < a.units) dw_unit(a, u, tile, c, c1);
     move(g);
@@ -343,7 +344,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
         const unsigned int r = tok0 + 2 * p + hi;
         const uint2 code = *reinterpret_cast<const uint2 *>(st + S::CODES + r * kTileI + l16 * 8);
         const unsigned int e = __shfl_sync(0xffffffffu, ex[p / 4], (2 * (p & 3) + hi) * 4 + (l16 >> 2));
-        *reinterpret_cast<uint4 *>(st + box + r * 128 + (((l16 & 7) ^ (r & 7)) << 4)) = dw_expand(code, e);
+        *reinterpret_cast<uint4 *>(st + box + r * 128 + (((l16 & 7) ^ (r & 7)) << 4)) = dw_expand(code, e, magic);
       }
       if (DY != DY_TMA) {
 #pragma unroll 1

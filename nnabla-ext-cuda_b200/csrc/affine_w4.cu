@@ -96,54 +96,96 @@ __global__ void __launch_bounds__(256)
 // subtraction leaves q - z, exactly. float32 rows are the exact sum of three bfloat16 parts, one instruction each. The products
 // of a group are summed by the tensor core (at most eight steps of 16, the small parts first), then scaled and added in fp32.
 
-template <typename T> struct W4Math {  // bfloat16, and float32 in parts
-  static constexpr unsigned int MAGIC = 0x43004300u;
+// For bfloat16 rows even that subtraction is left out: the instruction gets 128 + q, and (128 + z) times the group's sum of x -
+// one more pair of instructions with an operand of ones, shared by all output channels - is subtracted from the group's sum in
+// fp32. What that costs is the magnitude of the sums, about 30 times the result's: 5 of 24 bits, where the result keeps 8.
+
+template <typename T> struct W4Math {  // bfloat16; float32 in bfloat16 parts
+  static constexpr bool OFFSET = sizeof(T) == 2;  // the codes stay 128 above their value
+  static constexpr unsigned int MAGIC = 0x43004300u, ONES = 0x3f803f80u;
   static __device__ __forceinline__ unsigned int zero_pair(unsigned int z) { return (0x4300u + z) * 0x10001u; }
   static __device__ __forceinline__ unsigned int sub(unsigned int a, unsigned int b) {
+    if (OFFSET) return a;
     const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
     return *reinterpret_cast<const unsigned int *>(&r);
   }
+  // the pairs e = 0 1, 2 3, 4 5, 6 7 of a word, less the zero point
+  static __device__ __forceinline__ void unpack(unsigned int w, unsigned int z, unsigned int magic, unsigned int &p0, unsigned int &p1,
+                                                unsigned int &p2, unsigned int &p3) {
+    p0 = sub(and_or(w, 0x000f000fu, magic), z);
+    p1 = sub(and_or(w >> 4, 0x000f000fu, magic), z);
+    p2 = sub(and_or(w >> 8, 0x000f000fu, magic), z);
+    p3 = sub(and_or(w >> 12, 0x000f000fu, magic), z);
+  }
   static __device__ __forceinline__ void mma(float *c, const unsigned int *a, unsigned int b0, unsigned int b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 };
 template <> struct W4Math<__half> {
-  static constexpr unsigned int MAGIC = 0x64006400u;
+  static constexpr bool OFFSET = false;
+  static constexpr unsigned int MAGIC = 0x64006400u, ONES = 0x3c003c00u;
   static __device__ __forceinline__ unsigned int zero_pair(unsigned int z) { return (0x6400u + z) * 0x10001u; }
   static __device__ __forceinline__ unsigned int sub(unsigned int a, unsigned int b) {
     const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
     return *reinterpret_cast<const unsigned int *>(&r);
   }
+  // as above; the ten bits of the mantissa also take a code four bits higher, 1024 + 16 q, so that one shift does:
+  // (1024 + 16 q) / 16 - z' = q - z + 64 with z' = 1024 + z, less 960
+  static __device__ __forceinline__ unsigned int high(unsigned int a, unsigned int z) {
+    const unsigned int sixteenth = 0x2c002c00u, c960 = 0x63806380u;
+    const __half2 off = __hsub2(*reinterpret_cast<const __half2 *>(&c960), *reinterpret_cast<const __half2 *>(&z));
+    const __half2 q = __hfma2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&sixteenth), off);
+    return *reinterpret_cast<const unsigned int *>(&q);
+  }
+  static __device__ __forceinline__ void unpack(unsigned int w, unsigned int z, unsigned int magic, unsigned int &p0, unsigned int &p1,
+                                                unsigned int &p2, unsigned int &p3) {
+    const unsigned int w8 = w >> 8;
+    p0 = sub(and_or(w, 0x000f000fu, magic), z);
+    p1 = high(and_or(w, 0x00f000f0u, magic), z);
+    p2 = sub(and_or(w8, 0x000f000fu, magic), z);
+    p3 = high(and_or(w8, 0x00f000f0u, magic), z);
+  }
   static __device__ __forceinline__ void mma(float *c, const unsigned int *a, unsigned int b0, unsigned int b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 };
 
-// Eight consecutive elements of a row of x as the B operands of two instructions, part by part (float32: three bfloat16 parts).
+// Eight consecutive elements of a row of x: as they were loaded, and as the B operands of two instructions, part by part
+// (float32: three bfloat16 parts, heads by truncation and exact rests; an infinity has no rest, a NaN keeps one).
+template <typename T> struct XRaw {
+  uint4 w[8 * (int)sizeof(T) / 16];
+  __device__ __forceinline__ void load(const T *p, int n, bool vec) {  // n: elements that exist
+    if (vec) {
+#pragma unroll
+      for (int k = 0; k < 8 * (int)sizeof(T) / 16; ++k) w[k] = __ldg(reinterpret_cast<const uint4 *>(p) + k);
+    } else {
+      T e[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) e[k] = k < n ? __ldg(p + k) : Elem<T>::from_f32(0.0f);
+      memcpy(w, e, sizeof(w));
+    }
+  }
+};
 template <typename T> struct XFrag {
   static constexpr int PARTS = 1;
   unsigned int w[1][4];
-  __device__ __forceinline__ void set(const T *e) { memcpy(w[0], e, 16); }
-  __device__ __forceinline__ void load_vec(const T *p) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
-    w[0][0] = v.x; w[0][1] = v.y; w[0][2] = v.z; w[0][3] = v.w;
-  }
+  __device__ __forceinline__ explicit XFrag(const XRaw<T> &r) { w[0][0] = r.w[0].x; w[0][1] = r.w[0].y; w[0][2] = r.w[0].z; w[0][3] = r.w[0].w; }
 };
 template <> struct XFrag<float> {
   static constexpr int PARTS = 3;
   unsigned int w[3][4];
-  // heads by truncation, exact rests; an infinity has no rest (a NaN keeps one)
-  __device__ __forceinline__ void set(const float *e) {
+  __device__ __forceinline__ explicit XFrag(const XRaw<float> &r) {
+    const unsigned int e[8] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w, r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
     float v[8];
     unsigned int top = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      v[j] = e[j];
-      top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+      v[j] = __uint_as_float(e[j]);
+      top = max(top, e[j] & 0x7fffffffu);
     }
 #pragma unroll
     for (int q = 0; q < 3; ++q) {
@@ -157,14 +199,9 @@ template <> struct XFrag<float> {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const unsigned int half = j & 1 ? 0xffff0000u : 0xffffu;
-        if ((__float_as_uint(e[j]) & 0x7fffffffu) == 0x7f800000u) { w[1][j / 2] &= ~half; w[2][j / 2] &= ~half; }
+        if ((e[j] & 0x7fffffffu) == 0x7f800000u) { w[1][j / 2] &= ~half; w[2][j / 2] &= ~half; }
       }
     }
-  }
-  __device__ __forceinline__ void load_vec(const float *p) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-    const float e[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    set(e);
   }
 };
 
@@ -175,14 +212,15 @@ struct W4Args {
   long long ld_x, ld_y;
   int rows, c_in, c_out, i_tiles, o_tiles;
   int block;      // bytes of a packed block
-  int has_zeros;
-  int sums_at;    // where the sums lie in shared memory
-  int wk;         // warps along the input channels
+  int per_warp;   // blocks along the input channels per warp
+  int ring;       // copies in flight per warp and tile
+  int red_at, sums_at;  // where the sums lie in shared memory
   int vec;        // rows of x are 16-byte aligned
   int *flag;
 };
 
-constexpr int kRing = 4;  // blocks (times R) in flight per warp
+constexpr int kMaxRing = 2;  // copies in flight per warp: with 16 to 32 warps on an SM 64 to 130 KB, well above what latency x bandwidth asks for
+__host__ __device__ constexpr int w4_step(int R) { return R <= 2 ? 2 : 1; }  // blocks per copy
 
 __device__ __forceinline__ void w4_copy(void *dst, const void *src, unsigned int bytes, unsigned long long *bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
@@ -190,175 +228,216 @@ __device__ __forceinline__ void w4_copy(void *dst, const void *src, unsigned int
                : "memory");
 }
 
-// CTA: wo x wk warps; a warp has R tiles of 16 output channels and every wk-th tile of 128 input channels (of this CTA's share,
-// where a cluster of CTAs divides them); blockIdx.y: block of 8 NB rows of x. G: group size. Rows of x that do not exist are
-// read as row 0: their results are columns nobody stores.
-template <typename T, int G, int NB, int R>
+// Sum e of a group's accumulators (layout [R][NB][4][32 lanes]) to its place in y.
+template <typename T, int NB, int R>
+__device__ __forceinline__ void store_out(const W4Args &a, int og, int row0, int e, float v) {
+  const int l = e & 31, k = (e >> 5) & 3, n = (e >> 7) % NB, r = (e >> 7) / NB;
+  const int o = (og * R + r) * kTileO + (k >> 1) * 8 + (l >> 2), row = row0 + n * 8 + (l & 3) * 2 + (k & 1);
+  if (o < a.c_out && row < a.rows) {
+    if (a.b) v = __fadd_rn(v, Elem<T>::to_f32(__ldg(static_cast<const T *>(a.b) + o)));
+    static_cast<T *>(a.y)[(long long)row * a.ld_y + o] = Elem<T>::from_f32(v);
+  }
+}
+
+// A CTA takes R tiles of 16 output channels at a time (group blockIdx.x, then every n-th), its warps a run of per_warp tiles of
+// 128 input channels each (of the CTA's share, where a cluster of CTAs divides them). The copies run on from one group to the
+// next, so that memory is kept busy while the warps' sums are added. blockIdx.y: block of 8 NB rows of x. G: group size; ZEROS:
+// zero points. Rows of x that do not exist are read as row 0: their results are columns nobody stores.
+template <typename T, int G, int NB, int R, bool ZEROS>
 __global__ void __launch_bounds__(256) w4_affine_kernel(const W4Args a) {
   using M = W4Math<T>;
-  constexpr int PARTS = XFrag<T>::PARTS, GB = kTileI / G;  // groups per block
-  constexpr int PER_WARP = R * NB * 4 * 32;
+  constexpr int GB = kTileI / G;  // quantization groups per block
+  constexpr int BLOCK = kTileBytes + GB * kTileO * ((int)sizeof(T) + (ZEROS ? 1 : 0));
+  constexpr int PER_WARP = R * NB * 4 * 32, STEP = w4_step(R);
   extern __shared__ __align__(128) unsigned char w4_smem[];
-  __shared__ unsigned long long bars[8 * kRing];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, wo = warp / a.wk, wk = warp - wo * a.wk;
+  __shared__ unsigned long long bars[8 * kMaxRing];
+  const int lane = threadIdx.x & 31, wk = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int lr = lane >> 2, lc = lane & 3;
   unsigned int crank, csize;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(crank));
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
-  const int wos = warps / a.wk, ot0 = ((int)(blockIdx.x / csize) * wos + wo) * R;
+  const int og0 = blockIdx.x / csize, og_step = gridDim.x / csize, ogs = (a.o_tiles + R - 1) / R;
   const int row0 = blockIdx.y * 8 * NB;
-  const int stride = a.wk * (int)csize, first = wk + a.wk * (int)crank;
+  const int it0 = ((int)crank * warps + wk) * a.per_warp, blocks = max(0, min(a.i_tiles - it0, a.per_warp));
+  const int steps = (blocks + STEP - 1) / STEP;
   // each warp fills and empties a ring of its own: no other warp is waited for before the sums
-  unsigned char *ring = w4_smem + (size_t)warp * kRing * R * a.block;
-  unsigned long long *bar = bars + warp * kRing;
-  const int tiles = min(R, a.o_tiles - ot0);  // may be negative
-  const unsigned char *src = a.packed + ((long long)ot0 * a.i_tiles + first) * a.block;
+  unsigned char *ring = w4_smem + wk * a.ring * (R * STEP * BLOCK);
+  unsigned long long *bar = bars + wk * kMaxRing;
   if (lane == 0) {
-    for (int k = 0; k < kRing; ++k) mbar_init(&bar[k], 1);
+    for (int k = 0; k < a.ring; ++k) mbar_init(&bar[k], 1);
     mbar_fence_init();
   }
   __syncwarp();
+  // the first CTA's shared memory may only be written once it runs
+  if (csize > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
   pdl_launch_dependents();
   pdl_wait_for_predecessor();
-  auto fetch = [&](int it, int slot) {  // lane 0
-    mbar_expect_tx(&bar[slot], (unsigned)(tiles * a.block));
-    for (int r = 0; r < tiles; ++r)
-      w4_copy(ring + (size_t)(slot * R + r) * a.block, src + ((long long)r * a.i_tiles + (it - first)) * a.block, (unsigned)a.block, &bar[slot]);
+  const long long tile_bytes = (long long)a.i_tiles * BLOCK;
+  const unsigned char *src = a.packed + (long long)og0 * R * tile_bytes + (long long)it0 * BLOCK;  // of the next copy
+  int og_f = og0, step_f = 0, slot_f = 0;
+  auto fetch = [&]() {
+    if (og_f >= ogs || steps == 0) return;
+    if (elect_one()) {
+      const int tiles = min(R, a.o_tiles - og_f * R);
+      const unsigned int bytes = (unsigned)min(STEP, blocks - step_f * STEP) * BLOCK;
+      unsigned char *dst = ring + slot_f * (R * STEP * BLOCK);
+      mbar_expect_tx(&bar[slot_f], tiles * bytes);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (r < tiles) w4_copy(dst + r * (STEP * BLOCK), src + r * tile_bytes, bytes, &bar[slot_f]);
+    }
+    __syncwarp();
+    src += STEP * BLOCK;
+    if (++slot_f == a.ring) slot_f = 0;
+    if (++step_f == steps) {
+      step_f = 0;
+      og_f += og_step;
+      src += (long long)og_step * R * tile_bytes - (long long)steps * (STEP * BLOCK);
+    }
   };
-  if (lane == 0 && tiles > 0)
-    for (int k = 0; k < kRing && first + k * stride < a.i_tiles; ++k) fetch(first + k * stride, k);
-  const T *xr[NB];
+  for (int k = 0; k < a.ring; ++k) fetch();
+  const T *x0[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     const int row = row0 + n * 8 + lr;
-    xr[n] = static_cast<const T *>(a.x) + (long long)(row < a.rows ? row : 0) * a.ld_x + lc * 8;
+    x0[n] = static_cast<const T *>(a.x) + (long long)(row < a.rows ? row : 0) * a.ld_x + it0 * kTileI + lc * 8;
   }
-  float acc[R][NB][4];
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) acc[r][n][k] = 0.0f;
-  int slot = 0;
+  const unsigned int magic = opaque_constant(M::MAGIC);
+  const unsigned int ones[4] = {M::ONES, M::ONES, M::ONES, M::ONES};
+  const int i_left0 = a.c_in - it0 * kTileI - lc * 8;  // input channels from this lane's first one on
+  int slot = 0, buf = 0;
   unsigned int ph = 0;
   bool ok = true;
-  for (int it = first; tiles > 0 && it < a.i_tiles; it += stride) {
-    const int i0 = it * kTileI;
-    XFrag<T> x[4][NB];
-    if (a.vec && i0 + kTileI <= a.c_in) {
+  float *red = reinterpret_cast<float *>(w4_smem + a.red_at);    // [2][warp][R][NB][4][32]
+  float *sums = reinterpret_cast<float *>(w4_smem + a.sums_at);  // cluster: [2][CTA][PER_WARP], in the first CTA
+  for (int og = og0; og < ogs; og += og_step) {
+    float acc[R][NB][4];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[r][n][k] = 0.0f;
+    const unsigned char *blk = ring;
+    const T *xr[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) xr[n] = x0[n];
+    int i_left = i_left0;
+    for (int b = 0; ok && b < blocks; ++b) {
+      // the rows of x are asked for before the block's copy is waited for
+      XRaw<T> raw[4][NB];
+      const bool vec = a.vec && i_left >= kTileI - 24;  // whole block
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int n = 0; n < NB; ++n) x[j][n].load_vec(xr[n] + i0 + j * 32);
-    } else {
+        for (int n = 0; n < NB; ++n) raw[j][n].load(xr[n] + j * 32, i_left - j * 32, vec);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int n = 0; n < NB; ++n) xr[n] += kTileI;
+      i_left -= kTileI;
+      if (b % STEP == 0) {
+        blk = ring + slot * (R * STEP * BLOCK);
+        ok = pw_wait(&bar[slot], ph);
+        if (!ok) break;
+      }
+      float part[R][NB][4], xsum[NB][4];
+      uint4 lo4[R], hi4[R];
+      unsigned int z0[R], z1[R];
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          T e[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) e[k] = i0 + j * 32 + lc * 8 + k < a.c_in ? __ldg(xr[n] + i0 + j * 32 + k) : Elem<T>::from_f32(0.0f);
-          x[j][n].set(e);
-        }
-    }
-    ok = pw_wait(&bar[slot], ph);
-    if (!ok) break;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const unsigned char *blk = ring + (size_t)(slot * R + r) * a.block;  // a tile that does not exist is never copied: stale, and not stored
-      const uint4 lo4 = reinterpret_cast<const uint4 *>(blk)[lane], hi4 = reinterpret_cast<const uint4 *>(blk)[32 + lane];
-      float part[NB][4];
+      for (int r = 0; r < R; ++r) {  // a tile that does not exist is never copied: its slot is stale, its sums are not stored
+        lo4[r] = reinterpret_cast<const uint4 *>(blk + r * (STEP * BLOCK))[lane];
+        hi4[r] = reinterpret_cast<const uint4 *>(blk + r * (STEP * BLOCK))[32 + lane];
+        z0[r] = z1[r] = M::zero_pair(8);
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        constexpr int PER = G / 32;  // words per group
+        constexpr int PER = G / 32;  // words per quantization group
         const int g = j / PER;
-        unsigned int z0 = 8, z1 = 8;
-        if (a.has_zeros) {
-          const unsigned char *z = blk + kTileBytes + GB * kTileO * sizeof(T) + g * kTileO + lr;
-          z0 = z[0];
-          z1 = z[8];
-        }
-        z0 = M::zero_pair(z0);
-        z1 = M::zero_pair(z1);
-        if (j % PER == 0)
 #pragma unroll
-          for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) part[n][k] = 0.0f;
-        const unsigned int lo = j == 0 ? lo4.x : j == 1 ? lo4.y : j == 2 ? lo4.z : lo4.w;
-        const unsigned int hi = j == 0 ? hi4.x : j == 1 ? hi4.y : j == 2 ? hi4.z : hi4.w;
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          unsigned int f[4];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int sh = 4 * (2 * m + k);
-            f[2 * k] = M::sub(((lo >> sh) & 0x000f000fu) | M::MAGIC, z0);
-            f[2 * k + 1] = M::sub(((hi >> sh) & 0x000f000fu) | M::MAGIC, z1);
+        for (int n = 0; n < NB; ++n) {
+          const XFrag<T> x(raw[j][n]);
+          if (M::OFFSET) {  // every row of xsum is the group's sum of x
+            if (j % PER == 0) xsum[n][0] = xsum[n][1] = xsum[n][2] = xsum[n][3] = 0.0f;
+            M::mma(xsum[n], ones, x.w[0][0], x.w[0][1]);
+            M::mma(xsum[n], ones, x.w[0][2], x.w[0][3]);
           }
 #pragma unroll
-          for (int n = 0; n < NB; ++n)
+          for (int r = 0; r < R; ++r) {
+            const unsigned char *p = blk + r * (STEP * BLOCK);
+            if (j % PER == 0) {
+              if (ZEROS && n == 0) {
+                const unsigned char *z = p + kTileBytes + GB * kTileO * sizeof(T) + g * kTileO + lr;
+                z0[r] = M::zero_pair(z[0]);
+                z1[r] = M::zero_pair(z[8]);
+              }
 #pragma unroll
-            for (int q = PARTS - 1; q >= 0; --q) M::mma(part[n], f, x[j][n].w[q][2 * m], x[j][n].w[q][2 * m + 1]);
-        }
-        if (j % PER == PER - 1) {
-          const T *sc = reinterpret_cast<const T *>(blk + kTileBytes) + g * kTileO + lr;
-          const float s0 = Elem<T>::to_f32(sc[0]), s1 = Elem<T>::to_f32(sc[8]);
+              for (int k = 0; k < 4; ++k) part[r][n][k] = 0.0f;
+            }
+            const unsigned int lo = j == 0 ? lo4[r].x : j == 1 ? lo4[r].y : j == 2 ? lo4[r].z : lo4[r].w;
+            const unsigned int hi = j == 0 ? hi4[r].x : j == 1 ? hi4[r].y : j == 2 ? hi4[r].z : hi4[r].w;
+            unsigned int f[2][4];  // the same for every n: computed once
+            M::unpack(lo, z0[r], magic, f[0][0], f[0][2], f[1][0], f[1][2]);
+            M::unpack(hi, z1[r], magic, f[0][1], f[0][3], f[1][1], f[1][3]);
 #pragma unroll
-          for (int n = 0; n < NB; ++n)
+            for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) acc[r][n][k] = __fmaf_rn(part[n][k], k < 2 ? s0 : s1, acc[r][n][k]);
+              for (int q = XFrag<T>::PARTS - 1; q >= 0; --q) M::mma(part[r][n], f[m], x.w[q][2 * m], x.w[q][2 * m + 1]);
+            if (j % PER == PER - 1) {
+              const T *sc = reinterpret_cast<const T *>(p + kTileBytes) + g * kTileO + lr;
+              const float s0 = Elem<T>::to_f32(sc[0]), s1 = Elem<T>::to_f32(sc[8]);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                float v = part[r][n][k];
+                if (M::OFFSET) v = __fmaf_rn(xsum[n][k & 1], -__uint_as_float((k < 2 ? z0[r] : z1[r]) << 16), v);
+                acc[r][n][k] = __fmaf_rn(v, k < 2 ? s0 : s1, acc[r][n][k]);
+              }
+            }
+          }
         }
       }
+      blk += BLOCK;
+      if (b % STEP == STEP - 1 || b == blocks - 1) {
+        __syncwarp();  // every lane has read the slot
+        fetch();
+        if (++slot == a.ring) { slot = 0; ph ^= 1u; }
+      }
     }
-    __syncwarp();  // every lane has read the slot
-    if (lane == 0 && it + kRing * stride < a.i_tiles) fetch(it + kRing * stride, slot);
-    if (++slot == kRing) { slot = 0; ph ^= 1u; }
+    // the warps' sums (and then the CTAs') in a fixed order. One barrier per group and two buffers: whoever writes a buffer again
+    // has passed the barrier that the readers of its last contents reached after reading
+    float *mine = red + (buf * warps + wk) * PER_WARP;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mine[((r * NB + n) * 4 + k) * 32 + lane] = acc[r][n][k];
+    __syncthreads();
+    for (int e = threadIdx.x; e < PER_WARP; e += blockDim.x) {
+      const float *p = red + buf * warps * PER_WARP + e;
+      float v = p[0];
+      for (int k = 1; k < warps; ++k) v = __fadd_rn(v, p[k * PER_WARP]);
+      if (csize > 1) {
+        unsigned int to;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(smem_u32(sums + (buf * csize + crank) * PER_WARP + e)));
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
+      } else {
+        store_out<T, NB, R>(a, og, row0, e, v);
+      }
+    }
+    if (csize > 1) {
+      asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+      if (crank == 0)
+        for (int e = threadIdx.x; e < PER_WARP; e += blockDim.x) {
+          const float *p = sums + buf * csize * PER_WARP + e;
+          float v = p[0];
+          for (unsigned int k = 1; k < csize; ++k) v = __fadd_rn(v, p[k * PER_WARP]);
+          store_out<T, NB, R>(a, og, row0, e, v);
+        }
+    }
+    buf ^= 1;
   }
   if (!ok) {  // a copy did not land in time: recorded; the others in flight are given the same time before the ring goes away
     if (lane == 0) atomicExch(a.flag, 1);
-    for (int k = 1; k < kRing; ++k) pw_wait(&bar[(slot + k) % kRing], slot + k < kRing ? ph : ph ^ 1u);
-  }
-  __syncthreads();  // the rings have served; their memory takes the sums
-  float *red = reinterpret_cast<float *>(w4_smem);  // [warp][R][NB][4][32]
-  // the warps' sums (and then the CTAs') in a fixed order
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) red[warp * PER_WARP + ((r * NB + n) * 4 + k) * 32 + lane] = acc[r][n][k];
-  __syncthreads();
-  const int outs = wos * PER_WARP;
-  float *sums = reinterpret_cast<float *>(w4_smem + a.sums_at);  // cluster: [CTA][outs], in the first CTA
-  for (int e = threadIdx.x; e < outs; e += blockDim.x) {
-    const int o_w = e / PER_WARP, in = e - o_w * PER_WARP;
-    float v = 0.0f;
-    for (int k = 0; k < a.wk; ++k) v = __fadd_rn(v, red[(o_w * a.wk + k) * PER_WARP + in]);
-    if (csize > 1) {  // the first CTA's `sums` lies behind its own rings and sums, which it may still be using
-      unsigned int to;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"((unsigned)__cvta_generic_to_shared(sums + crank * outs + e)));
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
-    } else {
-      sums[e] = v;
-    }
-  }
-  if (csize > 1) {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (crank) return;
-  } else {
-    __syncthreads();
-  }
-  for (int e = threadIdx.x; e < outs; e += blockDim.x) {
-    float v = sums[e];
-    for (unsigned int k = 1; k < csize; ++k) v = __fadd_rn(v, sums[k * outs + e]);
-    const int l = e & 31, k = (e >> 5) & 3, n = (e >> 7) % NB, r = (e >> 7) / NB % R, o_w = e / PER_WARP;
-    const int o = (((int)(blockIdx.x / csize) * wos + o_w) * R + r) * kTileO + (k >> 1) * 8 + (l >> 2), row = row0 + n * 8 + (l & 3) * 2 + (k & 1);
-    if (o < a.c_out && row < a.rows) {
-      if (a.b) v = __fadd_rn(v, Elem<T>::to_f32(__ldg(static_cast<const T *>(a.b) + o)));
-      static_cast<T *>(a.y)[(long long)row * a.ld_y + o] = Elem<T>::from_f32(v);
-    }
+    for (int k = 1; k < a.ring; ++k) pw_wait(&bar[(slot + k) % a.ring], slot + k < a.ring ? ph : ph ^ 1u);
   }
 }
 
@@ -385,21 +464,23 @@ int pack_t(const dwbnq_w4_desc &d, const void *codes, const void *scales, const 
                                    static_cast<unsigned char *>(packed));
   return e == cudaSuccess ? DWBNQ_OK : fail_cuda(e, "w4_pack_kernel launch");
 }
-template <typename T, int G, int NB, int R>
-int affine_launch(W4Args a, int wo, int wk, int cluster, cudaStream_t stream) {
-  a.wk = wk;
-  const int per_warp = R * NB * 4 * 32, o_ctas = (a.o_tiles + wo * R - 1) / (wo * R);
-  const size_t rings = (size_t)wo * wk * kRing * R * a.block, own = sizeof(float) * (size_t)per_warp * wo * wk;
-  a.sums_at = (int)((rings > own ? rings : own) + 15) / 16 * 16;
-  const size_t smem = a.sums_at + sizeof(float) * (size_t)per_warp * cluster * wo;
-  auto kern = w4_affine_kernel<T, G, NB, R>;
-  if (smem > 48 * 1024) {
+template <typename T, int G, int NB, int R, bool ZEROS>
+int affine_launch(W4Args a, int warps, int cluster, int ctas, cudaStream_t stream) {
+  a.per_warp = (a.i_tiles + warps * cluster - 1) / (warps * cluster);
+  const int per_warp = R * NB * 4 * 32, ogs = (a.o_tiles + R - 1) / R;
+  const int steps = (a.per_warp + w4_step(R) - 1) / w4_step(R), rounds = (ogs + ctas - 1) / ctas;
+  a.ring = steps * rounds < kMaxRing ? steps * rounds : kMaxRing;
+  a.red_at = (warps * a.ring * w4_step(R) * R * a.block + 15) / 16 * 16;
+  a.sums_at = a.red_at + 2 * warps * per_warp * (int)sizeof(float);
+  const size_t smem = a.sums_at + (cluster > 1 ? 2 * sizeof(float) * (size_t)per_warp * cluster : 0);
+  auto kern = w4_affine_kernel<T, G, NB, R, ZEROS>;
+  if (smem > 40 * 1024) {  // above 48 KB with the static part
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return fail_cuda(e, "w4_affine_kernel attributes");
   }
   cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3((unsigned)(o_ctas * cluster), (unsigned)((a.rows + 8 * NB - 1) / (8 * NB)));
-  lc.blockDim = dim3((unsigned)(32 * wo * wk));
+  lc.gridDim = dim3((unsigned)((ogs + rounds - 1) / rounds * cluster), (unsigned)((a.rows + 8 * NB - 1) / (8 * NB)));
+  lc.blockDim = dim3((unsigned)(32 * warps));
   lc.dynamicSmemBytes = smem;
   lc.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -413,16 +494,26 @@ int affine_launch(W4Args a, int wo, int wk, int cluster, cudaStream_t stream) {
   const cudaError_t e = cudaLaunchKernelEx(&lc, kern, a);
   return e == cudaSuccess ? DWBNQ_OK : fail_cuda(e, "w4_affine_kernel launch");
 }
-template <typename T, int G>
+// Output tiles per warp: a warp's rows of x, its waits and its loop cost the same for one tile and for four, so with enough work
+// for every SM (27 blocks) a warp takes as many as its registers allow (4096 -> 14336, one bf16 row: 16.0 us with one, 12.7 with
+// two, 11.4 with four); with less, one, so that more warps share it (512 -> 512: 2.1 us against 3.1). The grid is what then stays
+// resident; where the output tiles are too few for it, a cluster of CTAs divides the input channels of each.
+template <typename T, int G, bool ZEROS>
 int affine_g(const W4Args &a, cudaStream_t stream) {
-  const int nb = a.rows > 8 ? 2 : 1;
-  int wo = 1, wk = 8, cluster = 1;
-  if (nb == 2) { wo = 2; wk = 4; }
-  while (wk > 1 && wk > a.i_tiles) wk >>= 1;
-  const int R = nb == 2 ? 2 : 1;
-  const int o_ctas = (a.o_tiles + wo * R - 1) / (wo * R);
-  while (cluster < 8 && o_ctas * cluster * 2 <= kPlanSms && a.i_tiles >= 2 * cluster * wk) cluster *= 2;
-  return nb == 2 ? affine_launch<T, G, 2, 2>(a, wo, wk, cluster, stream) : affine_launch<T, G, 1, 1>(a, wo, wk, cluster, stream);
+  constexpr int WIDE1 = sizeof(T) == 2 ? 4 : 2, WIDE2 = 2;
+  const bool many = (long long)a.o_tiles * a.i_tiles >= 27LL * kPlanSms;
+  const int nb = a.rows > 8 ? 2 : 1, R = !many ? 1 : nb == 2 ? WIDE2 : WIDE1, ogs = (a.o_tiles + R - 1) / R;
+  const int resident = (R == 4 ? 2 : R == 2 ? 3 : 4) * kPlanSms;
+  int warps = 8, cluster = 1;
+  while (warps > 1 && warps > a.i_tiles) warps >>= 1;
+  while (cluster < 8 && ogs * cluster * 2 <= resident && a.i_tiles >= 2 * cluster * warps) cluster *= 2;
+  const int ctas = resident / cluster;
+  if (nb == 2) return many ? affine_launch<T, G, 2, WIDE2, ZEROS>(a, warps, cluster, ctas, stream) : affine_launch<T, G, 2, 1, ZEROS>(a, warps, cluster, ctas, stream);
+  return many ? affine_launch<T, G, 1, WIDE1, ZEROS>(a, warps, cluster, ctas, stream) : affine_launch<T, G, 1, 1, ZEROS>(a, warps, cluster, ctas, stream);
+}
+template <typename T, int G>
+int affine_z(const W4Args &a, bool zeros, cudaStream_t stream) {
+  return zeros ? affine_g<T, G, true>(a, stream) : affine_g<T, G, false>(a, stream);
 }
 template <typename T>
 int affine_t(const dwbnq_w4_desc &d, long long rows, long long ld_x, const void *x, const void *packed, const void *b,
@@ -433,11 +524,12 @@ int affine_t(const dwbnq_w4_desc &d, long long rows, long long ld_x, const void 
   if (st != DWBNQ_OK) return st;
   a.x = x; a.b = b; a.y = y;
   a.packed = static_cast<const unsigned char *>(packed);
-  a.block = l.block; a.has_zeros = d.has_zeros;
+  a.block = l.block;
   a.ld_x = ld_x; a.ld_y = ld_y;
   a.rows = (int)rows; a.c_in = d.c_in; a.c_out = d.c_out; a.i_tiles = (int)l.i_tiles; a.o_tiles = (int)l.o_tiles;
   a.vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_x * sizeof(T) % 16 == 0;
-  return d.group == 32 ? affine_g<T, 32>(a, stream) : d.group == 64 ? affine_g<T, 64>(a, stream) : affine_g<T, 128>(a, stream);
+  const bool z = d.has_zeros != 0;
+  return d.group == 32 ? affine_z<T, 32>(a, z, stream) : d.group == 64 ? affine_z<T, 64>(a, z, stream) : affine_z<T, 128>(a, z, stream);
 }
 
 }  // namespace

@@ -48,6 +48,18 @@ __device__ __forceinline__ bool pw_wait(unsigned long long *bar, unsigned int pa
   }
   return ok;
 }
+// (a & mask) | set as one instruction. A logic instruction takes one immediate: with both constants known the compiler needs two,
+// so `set` has to come from a value it cannot see through (opaque_constant).
+__device__ __forceinline__ unsigned int and_or(unsigned int a, unsigned int mask, unsigned int set) {
+  unsigned int r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(mask), "r"(set));
+  return r;
+}
+__device__ __forceinline__ unsigned int opaque_constant(unsigned int v) {
+  unsigned int r;
+  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 // True in one lane of a converged warp. TMA and tcgen05 instructions take their operands from uniform registers: issued under this
 // predicate from code the whole warp walks through, addresses and descriptors stay there; issued under `lane == 0` every
 // operand is moved over one instruction at a time (the MMA thread of the weight gradient: 1400 cycles per four MMAs against 600).
