@@ -44,10 +44,126 @@ __device__ __forceinline__ float ck_inv_step(unsigned int b) {
 __device__ __forceinline__ float ck_step(unsigned int b) {
   return b == kCkNonFinite ? __uint_as_float(0x7fc00000u) : __uint_as_float((b - 6u) << 23);
 }
-__device__ __forceinline__ int ck_code(float x, float inv) {
-  // fminf / fmaxf drop the NaN that a value that is not finite leaves (0 * inf): code 0 by the last select
-  const float t = fminf(fmaxf(__fmul_rn(x, inv), -127.0f), 127.0f);
-  return inv == 0.0f ? 0 : __float2int_rn(t);
+// ---- eight consecutive values of a row: what a lane works on; four lanes share a group -----------------------
+
+// How a row of a tensor may be accessed: 16-byte vectors, 4-byte words (two 16-bit values, one fp32), or single values. The
+// same for every row, from the tensor's address and row stride.
+enum OctetAccess : int { OCTET_VALUE = 0, OCTET_WORD = 1, OCTET_VECTOR = 2 };
+inline int octet_access(const void *p, long long ld, int bytes) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * bytes);
+  return a % 16 == 0 ? OCTET_VECTOR : a % 4 == 0 ? OCTET_WORD : OCTET_VALUE;
+}
+template <typename T> struct Octet {
+  static constexpr int VECS = 8 * (int)sizeof(T) / 16, WORDS = 8 * (int)sizeof(T) / 4;
+  // n: values that exist (the rest are 0); p is not followed for n <= 0
+  static __device__ __forceinline__ void load(const T *p, long long n, int access, float *v) {
+    T e[8];
+    if (n >= 8 && access == OCTET_VECTOR) {
+      uint4 w[VECS];
+#pragma unroll
+      for (int k = 0; k < VECS; ++k) w[k] = __ldcs(reinterpret_cast<const uint4 *>(p) + k);
+      memcpy(e, w, sizeof(e));
+    } else if (n >= 8 && access == OCTET_WORD) {
+      unsigned int w[WORDS];
+#pragma unroll
+      for (int k = 0; k < WORDS; ++k) w[k] = __ldg(reinterpret_cast<const unsigned int *>(p) + k);
+      memcpy(e, w, sizeof(e));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) e[k] = k < n ? p[k] : Elem<T>::from_f32(0.0f);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = Elem<T>::to_f32(e[k]);
+  }
+  static __device__ __forceinline__ void store(T *p, long long n, int access, const float *v) {
+    T e[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) e[k] = Elem<T>::from_f32(v[k]);
+    if (n >= 8 && access == OCTET_VECTOR) {
+      uint4 w[VECS];
+      memcpy(w, e, sizeof(e));
+#pragma unroll
+      for (int k = 0; k < VECS; ++k) __stcs(reinterpret_cast<uint4 *>(p) + k, w[k]);
+    } else if (n >= 8 && access == OCTET_WORD) {
+      unsigned int w[WORDS];
+      memcpy(w, e, sizeof(e));
+#pragma unroll
+      for (int k = 0; k < WORDS; ++k) reinterpret_cast<unsigned int *>(p)[k] = w[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < n) p[k] = e[k];
+    }
+  }
+};
+
+// A walk over all octets of [rows, 4 * groups]: thread t of the grid starts at octet t and goes on by the grid's size, with one
+// division at the start. A warp's lanes stay together: whole groups, and so whole warps of shuffles, as the totals are multiples of 4
+// and lanes past the end take part with `in` false.
+struct OctetWalk {
+  long long row, rows, row_step;
+  unsigned int col, per_row, col_step;  // octets
+};
+struct OctetGrid {  // host: the grid and its step
+  unsigned int ctas;
+  long long row_step;
+  unsigned int col_step, per_row;
+};
+inline OctetGrid octet_grid(long long rows, long long cols, int threads, int max_ctas) {
+  OctetGrid g;
+  g.per_row = (unsigned int)((cols + kCkGroup - 1) / kCkGroup * 4);
+  const long long total = rows * g.per_row, need = (total + threads - 1) / threads;
+  g.ctas = (unsigned int)(need < max_ctas ? need : max_ctas);
+  const long long step = (long long)g.ctas * threads;
+  g.row_step = step / g.per_row;
+  g.col_step = (unsigned int)(step % g.per_row);
+  return g;
+}
+__device__ __forceinline__ OctetWalk octet_walk(const OctetGrid &g, long long rows) {
+  OctetWalk w;
+  const long long first = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  w.row = first / g.per_row;
+  w.col = (unsigned int)(first - w.row * g.per_row);
+  w.rows = rows; w.row_step = g.row_step; w.per_row = g.per_row; w.col_step = g.col_step;
+  return w;
+}
+__device__ __forceinline__ void octet_next(OctetWalk &w) {
+  w.row += w.row_step;
+  w.col += w.col_step;
+  if (w.col >= w.per_row) { w.col -= w.per_row; ++w.row; }
+}
+
+// Writes the checkpoint of a lane's eight values; the four lanes of a group work together (all lanes of the warp call it).
+__device__ __forceinline__ void ck_put(const float *v, bool in, long long octet, signed char *codes, unsigned char *exps) {
+  unsigned int m = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  const unsigned int b = ck_exponent(m);
+  const float inv = ck_inv_step(b);
+  // x / delta + 1.5 * 2^23 rounds to the integer, half to even, and leaves it in the low byte; a NaN (0 * inf, in a group that is
+  // not finite) is dropped by the maximum
+  unsigned int w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    unsigned int t[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) t[k] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fmul_rn(v[4 * h + k], inv), -127.0f), 127.0f), 12582912.0f));
+    w[h] = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+  }
+  if (inv == 0.0f) w[0] = w[1] = 0u;
+  if (in) {
+    __stcs(reinterpret_cast<uint2 *>(codes) + octet, make_uint2(w[0], w[1]));
+    if ((threadIdx.x & 3) == 0) exps[octet >> 2] = (unsigned char)b;
+  }
+}
+// Reads them back (0 for lanes past the end).
+__device__ __forceinline__ void ck_get(const signed char *codes, const unsigned char *exps, bool in, long long octet, float *v) {
+  const uint2 c = in ? __ldcs(reinterpret_cast<const uint2 *>(codes) + octet) : make_uint2(0u, 0u);
+  const float step = ck_step(in ? __ldg(exps + (octet >> 2)) : kCkMinExp);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = __fmul_rn((float)(signed char)((k < 4 ? c.x : c.y) >> (8 * (k & 3))), step);
 }
 
 }  // namespace dwbnq

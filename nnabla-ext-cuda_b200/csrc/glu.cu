@@ -13,22 +13,28 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <int ACT>
+// For 16-bit tensors the exponential and the division are the hardware's approximations (a few 2^-23, the exponential
+// 2 + 1.2 |g| of them): the result keeps 8 or 11 bits.
+template <typename T> __device__ __forceinline__ float glu_sigmoid(float g) {
+  if (sizeof(T) == 4) return __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-g)));
+  return __fdividef(1.0f, __fadd_rn(1.0f, __expf(-g)));
+}
+template <typename T, int ACT>
 __device__ __forceinline__ float act_value(float g) {
-  if (ACT == DWBNQ_ACT_SILU) return __fdiv_rn(g, __fadd_rn(1.0f, expf(-g)));
+  if (ACT == DWBNQ_ACT_SILU) return __fmul_rn(g, glu_sigmoid<T>(g));
   if (ACT == DWBNQ_ACT_GELU) return __fmul_rn(g, __fmul_rn(0.5f, erfcf(__fmul_rn(g, -0.70710678118654752f))));
   return g > 0.0f ? g : (g != g ? g : 0.0f);
 }
-template <int ACT>
+template <typename T, int ACT>
 __device__ __forceinline__ void act_both(float g, float &a, float &d) {
   if (ACT == DWBNQ_ACT_SILU) {
-    const float s = __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-g)));
+    const float s = glu_sigmoid<T>(g);
     a = __fmul_rn(g, s);
     d = __fmul_rn(s, __fmaf_rn(g, __fsub_rn(1.0f, s), 1.0f));
   } else if (ACT == DWBNQ_ACT_GELU) {
-    const float p = __fmul_rn(0.5f, erfcf(__fmul_rn(g, -0.70710678118654752f)));
+    const float p = __fmul_rn(0.5f, erfcf(__fmul_rn(g, -0.70710678118654752f))), t = __fmul_rn(__fmul_rn(g, -0.5f), g);
     a = __fmul_rn(g, p);
-    d = __fmaf_rn(__fmul_rn(g, 0.39894228040143268f), expf(__fmul_rn(__fmul_rn(g, -0.5f), g)), p);
+    d = __fmaf_rn(__fmul_rn(g, 0.39894228040143268f), sizeof(T) == 4 ? expf(t) : __expf(t), p);
   } else {
     a = g > 0.0f ? g : (g != g ? g : 0.0f);
     d = g > 0.0f ? 1.0f : (g != g ? g : 0.0f);
@@ -38,93 +44,104 @@ __device__ __forceinline__ void act_both(float g, float &a, float &d) {
 struct GluFwdArgs {
   const void *gate, *up;
   void *y;
-  long long ld_gate, ld_up, ld_y, rows, cols, groups;
+  long long ld_gate, ld_up, ld_y, rows, cols;
   signed char *gate_codes, *up_codes;  // null: no checkpoints
   unsigned char *gate_exps, *up_exps;
+  int acc_gate, acc_up, acc_y;  // OctetAccess
+  OctetGrid grid;
 };
 struct GluBwdArgs {
   const signed char *gate_codes, *up_codes;
   const unsigned char *gate_exps, *up_exps;
   const void *dy;
   void *dgate, *dup;  // either may be null
-  long long ld_dy, ld_dgate, ld_dup, rows, cols, groups;
+  long long ld_dy, ld_dgate, ld_dup, rows, cols;
   signed char *prod_codes;  // null: the product is not wanted
   unsigned char *prod_exps;
   int accum;  // bit 0 dgate, bit 1 dup
+  int acc_dy, acc_dgate, acc_dup;
+  OctetGrid grid;
 };
 
-__device__ __forceinline__ void put_group(float v, long long g, int lane, signed char *codes, unsigned char *exps) {
-  const unsigned int b = ck_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
-  codes[g * kCkGroup + lane] = (signed char)ck_code(v, ck_inv_step(b));
-  if (lane == 0) exps[g] = (unsigned char)b;
-}
-
-// One warp per group of 32 values, one lane per value.
-template <typename T, int ACT>
+template <typename T, int ACT, bool CKPT>
 __global__ void __launch_bounds__(kThreads) glu_fwd_kernel(const GluFwdArgs a) {
   pdl_launch_dependents();
   pdl_wait_for_predecessor();
-  const int lane = threadIdx.x & 31;
-  const long long total = a.rows * a.groups, step = (long long)gridDim.x * (kThreads / 32);
-  for (long long g = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); g < total; g += step) {
-    const long long r = g / a.groups, c = (g - r * a.groups) * kCkGroup + lane;
-    float vg = 0.0f, vu = 0.0f;
-    if (c < a.cols) {
-      vg = Elem<T>::to_f32(static_cast<const T *>(a.gate)[r * a.ld_gate + c]);
-      vu = Elem<T>::to_f32(static_cast<const T *>(a.up)[r * a.ld_up + c]);
-      static_cast<T *>(a.y)[r * a.ld_y + c] = Elem<T>::from_f32(__fmul_rn(act_value<ACT>(vg), vu));
-    }
-    if (a.gate_codes) {
-      put_group(vg, g, lane, a.gate_codes, a.gate_exps);
-      put_group(vu, g, lane, a.up_codes, a.up_exps);
+  for (OctetWalk w = octet_walk(a.grid, a.rows); __any_sync(0xffffffffu, w.row < a.rows); octet_next(w)) {
+    const bool in = w.row < a.rows;
+    const long long c = w.col * 8LL, n = in ? a.cols - c : 0;
+    float g[8], u[8], y[8];
+    Octet<T>::load(static_cast<const T *>(a.gate) + w.row * a.ld_gate + c, n, a.acc_gate, g);
+    Octet<T>::load(static_cast<const T *>(a.up) + w.row * a.ld_up + c, n, a.acc_up, u);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y[k] = __fmul_rn(act_value<T, ACT>(g[k]), u[k]);
+    Octet<T>::store(static_cast<T *>(a.y) + w.row * a.ld_y + c, n, a.acc_y, y);
+    if (CKPT) {
+      ck_put(g, in, w.row * w.per_row + w.col, a.gate_codes, a.gate_exps);
+      ck_put(u, in, w.row * w.per_row + w.col, a.up_codes, a.up_exps);
     }
   }
+}
+
+template <typename T>
+__device__ __forceinline__ void put_gradient(T *p, long long n, int access, bool accum, float *v) {
+  if (accum) {
+    float old[8];
+    Octet<T>::load(p, n, access, old);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = __fadd_rn(old[k], v[k]);
+  }
+  Octet<T>::store(p, n, access, v);
 }
 
 template <typename T, int ACT>
 __global__ void __launch_bounds__(kThreads) glu_bwd_kernel(const GluBwdArgs a) {
   pdl_launch_dependents();
   pdl_wait_for_predecessor();
-  const int lane = threadIdx.x & 31;
-  const long long total = a.rows * a.groups, step = (long long)gridDim.x * (kThreads / 32);
-  for (long long g = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); g < total; g += step) {
-    const long long r = g / a.groups, c = (g - r * a.groups) * kCkGroup + lane;
-    const float vg = __fmul_rn((float)a.gate_codes[g * kCkGroup + lane], ck_step(a.gate_exps[g]));
-    const float vu = __fmul_rn((float)a.up_codes[g * kCkGroup + lane], ck_step(a.up_exps[g]));
-    float act, der;
-    act_both<ACT>(vg, act, der);
-    if (c < a.cols) {
-      const float dy = a.dy ? Elem<T>::to_f32(static_cast<const T *>(a.dy)[r * a.ld_dy + c]) : 0.0f;
-      if (a.dgate) {
-        T *p = static_cast<T *>(a.dgate) + r * a.ld_dgate + c;
-        float v = __fmul_rn(__fmul_rn(dy, vu), der);
-        if (a.accum & 1) v = __fadd_rn(Elem<T>::to_f32(*p), v);
-        *p = Elem<T>::from_f32(v);
-      }
-      if (a.dup) {
-        T *p = static_cast<T *>(a.dup) + r * a.ld_dup + c;
-        float v = __fmul_rn(dy, act);
-        if (a.accum & 2) v = __fadd_rn(Elem<T>::to_f32(*p), v);
-        *p = Elem<T>::from_f32(v);
-      }
+  for (OctetWalk w = octet_walk(a.grid, a.rows); __any_sync(0xffffffffu, w.row < a.rows); octet_next(w)) {
+    const bool in = w.row < a.rows;
+    const long long c = w.col * 8LL, n = in ? a.cols - c : 0, at = w.row * w.per_row + w.col;
+    float g[8], u[8], dy[8], t[8], d[8];
+    ck_get(a.gate_codes, a.gate_exps, in, at, g);
+    ck_get(a.up_codes, a.up_exps, in, at, u);
+    Octet<T>::load(static_cast<const T *>(a.dy) + w.row * a.ld_dy + c, a.dy ? n : 0, a.acc_dy, dy);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) act_both<T, ACT>(g[k], t[k], d[k]);
+    if (a.dgate) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) d[k] = __fmul_rn(__fmul_rn(dy[k], u[k]), d[k]);
+      put_gradient(static_cast<T *>(a.dgate) + w.row * a.ld_dgate + c, n, a.acc_dgate, (a.accum & 1) != 0, d);
     }
-    if (a.prod_codes) put_group(c < a.cols ? __fmul_rn(act, vu) : 0.0f, g, lane, a.prod_codes, a.prod_exps);
+    if (a.dup) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) dy[k] = __fmul_rn(dy[k], t[k]);
+      put_gradient(static_cast<T *>(a.dup) + w.row * a.ld_dup + c, n, a.acc_dup, (a.accum & 2) != 0, dy);
+    }
+    if (a.prod_codes) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) t[k] = k < n ? __fmul_rn(t[k], u[k]) : 0.0f;
+      ck_put(t, in, at, a.prod_codes, a.prod_exps);
+    }
   }
 }
 
-unsigned int grid_for(long long warps) {
-  const long long blocks = (warps + kThreads / 32 - 1) / (kThreads / 32), cap = (long long)sm_count(-1) * 16;
-  return (unsigned int)(blocks > cap ? cap : blocks < 1 ? 1 : blocks);
-}
-
 template <typename T, int ACT>
-int fwd_t(const GluFwdArgs &a, cudaStream_t stream) {
-  const cudaError_t e = launch_pdl(glu_fwd_kernel<T, ACT>, dim3(grid_for(a.rows * a.groups)), dim3(kThreads), 0, stream, a);
+int fwd_t(GluFwdArgs a, cudaStream_t stream) {
+  a.grid = octet_grid(a.rows, a.cols, kThreads, sm_count(-1) * 8);
+  a.acc_gate = octet_access(a.gate, a.ld_gate, sizeof(T));
+  a.acc_up = octet_access(a.up, a.ld_up, sizeof(T));
+  a.acc_y = octet_access(a.y, a.ld_y, sizeof(T));
+  const cudaError_t e = a.gate_codes ? launch_pdl(glu_fwd_kernel<T, ACT, true>, dim3(a.grid.ctas), dim3(kThreads), 0, stream, a)
+                                     : launch_pdl(glu_fwd_kernel<T, ACT, false>, dim3(a.grid.ctas), dim3(kThreads), 0, stream, a);
   return e == cudaSuccess ? DWBNQ_OK : fail_cuda(e, "glu_fwd_kernel launch");
 }
 template <typename T, int ACT>
-int bwd_t(const GluBwdArgs &a, cudaStream_t stream) {
-  const cudaError_t e = launch_pdl(glu_bwd_kernel<T, ACT>, dim3(grid_for(a.rows * a.groups)), dim3(kThreads), 0, stream, a);
+int bwd_t(GluBwdArgs a, cudaStream_t stream) {
+  a.grid = octet_grid(a.rows, a.cols, kThreads, sm_count(-1) * 8);
+  a.acc_dy = octet_access(a.dy, a.ld_dy, sizeof(T));
+  a.acc_dgate = octet_access(a.dgate, a.ld_dgate, sizeof(T));
+  a.acc_dup = octet_access(a.dup, a.ld_dup, sizeof(T));
+  const cudaError_t e = launch_pdl(glu_bwd_kernel<T, ACT>, dim3(a.grid.ctas), dim3(kThreads), 0, stream, a);
   return e == cudaSuccess ? DWBNQ_OK : fail_cuda(e, "glu_bwd_kernel launch");
 }
 template <typename T>
@@ -143,10 +160,10 @@ int bwd_act(int act, const GluBwdArgs &a, cudaStream_t s) {
 int launch_glu_fwd(int dtype, int act, long long rows, long long cols, long long ld_gate, const void *gate, long long ld_up,
                    const void *up, long long ld_y, void *y, void *gate_codes, void *gate_exps, void *up_codes, void *up_exps,
                    cudaStream_t stream) {
-  GluFwdArgs a;
+  GluFwdArgs a = {};
   a.gate = gate; a.up = up; a.y = y;
   a.ld_gate = ld_gate; a.ld_up = ld_up; a.ld_y = ld_y;
-  a.rows = rows; a.cols = cols; a.groups = (cols + kCkGroup - 1) / kCkGroup;
+  a.rows = rows; a.cols = cols;
   a.gate_codes = static_cast<signed char *>(gate_codes); a.up_codes = static_cast<signed char *>(up_codes);
   a.gate_exps = static_cast<unsigned char *>(gate_exps); a.up_exps = static_cast<unsigned char *>(up_exps);
   if (dtype == DWBNQ_F32) return fwd_act<float>(act, a, stream);
@@ -157,12 +174,12 @@ int launch_glu_fwd(int dtype, int act, long long rows, long long cols, long long
 int launch_glu_bwd(int dtype, int act, long long rows, long long cols, const void *gate_codes, const void *gate_exps,
                    const void *up_codes, const void *up_exps, long long ld_dy, const void *dy, long long ld_dgate, void *dgate,
                    long long ld_dup, void *dup, void *prod_codes, void *prod_exps, int accum, cudaStream_t stream) {
-  GluBwdArgs a;
+  GluBwdArgs a = {};
   a.gate_codes = static_cast<const signed char *>(gate_codes); a.up_codes = static_cast<const signed char *>(up_codes);
   a.gate_exps = static_cast<const unsigned char *>(gate_exps); a.up_exps = static_cast<const unsigned char *>(up_exps);
   a.dy = dy; a.dgate = dgate; a.dup = dup;
   a.ld_dy = ld_dy; a.ld_dgate = ld_dgate; a.ld_dup = ld_dup;
-  a.rows = rows; a.cols = cols; a.groups = (cols + kCkGroup - 1) / kCkGroup;
+  a.rows = rows; a.cols = cols;
   a.prod_codes = static_cast<signed char *>(prod_codes); a.prod_exps = static_cast<unsigned char *>(prod_exps);
   a.accum = accum;
   if (dtype == DWBNQ_F32) return bwd_act<float>(act, a, stream);
