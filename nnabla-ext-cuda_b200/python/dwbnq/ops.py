@@ -334,17 +334,46 @@ def _one_device(*ts):
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise ValueError("dwbnq operators take CUDA tensors (there is no CPU fallback)")
-        if dev is not None and t.device != dev:
-            raise ValueError("all tensors must live on one device")
-        dev = t.device
+        d = t.device
+        if d != dev:
+            if not t.is_cuda:
+                raise ValueError("dwbnq operators take CUDA tensors (there is no CPU fallback)")
+            if dev is not None:
+                raise ValueError("all tensors must live on one device")
+            dev = d
     return dev
+
+
+def _launch(name, dev, *args):
+    """Calls an entry point of the library on dev's current stream, with dev current for the call only. These operators are called
+    thousands of times a second by a serving loop: the common case makes no context object and wraps no pointer."""
+    fn = getattr(L.lib(), name)
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        status = fn(*args, index, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, index, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        L.check(status)
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _rows_view(t, name):
     """(rows, cols, row stride) of [..., cols] seen as a matrix."""
-    if t.dim() < 1:
+    dim = t.dim()
+    if dim == 2 or (dim > 0 and t.is_contiguous()):
+        cols = t.shape[-1]
+        if dim == 2:
+            rows, (ld, unit) = t.shape[0], t.stride()
+            if rows > 1 and cols > 0 and unit == 1 and ld >= cols:
+                return rows, cols, ld
+        elif cols > 0:
+            return t.numel() // cols, cols, cols
+    if dim < 1:
         raise ValueError("%s must have at least one axis" % name)
     cols = int(t.shape[-1])
     rows = 1
@@ -369,11 +398,11 @@ def _rows_view(t, name):
     return rows, cols, max(ld, cols)
 
 
-def _like(t, name, shape, dtype, device, written=False):
+def _like(t, name, shape, dtype, device):
     """A given output (or a second input) checked against what it has to be; a new one when it is None."""
     if t is None:
         return torch.empty(shape, dtype=dtype, device=device)
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+    if t.shape != shape or t.dtype != dtype:
         raise ValueError("%s must be %s of shape %s, got %s of shape %s" % (name, dtype, tuple(shape), t.dtype, tuple(t.shape)))
     return t
 
@@ -399,13 +428,15 @@ class Code8Checkpoint:
 
     @classmethod
     def empty(cls, shape, dtype, device):
-        shape = tuple(int(s) for s in shape)
+        ck = cls.__new__(cls)
         rows = 1
         for s in shape[:-1]:
             rows *= s
         groups = (shape[-1] + CODE8_GROUP - 1) // CODE8_GROUP
-        return cls(torch.empty((rows, CODE8_GROUP * groups), dtype=torch.int8, device=device),
-                   torch.empty((rows, groups), dtype=torch.uint8, device=device), shape, dtype)
+        ck.codes = torch.empty((rows, CODE8_GROUP * groups), dtype=torch.int8, device=device)
+        ck.exponents = torch.empty((rows, groups), dtype=torch.uint8, device=device)
+        ck.shape, ck.dtype, ck.rows, ck.cols = tuple(shape), dtype, rows, shape[-1]
+        return ck
 
 
 def _ck_out(ck, name, shape, dtype, device):
@@ -422,9 +453,7 @@ def checkpoint_code8(x, out=None):
     ck = _ck_out(out, "out", x.shape, x.dtype, x.device)
     dev = _one_device(x, ck.codes, ck.exponents)
     rows, cols, ld = _rows_view(x, "x")
-    with torch.cuda.device(dev):
-        L.check(L.lib().dwbnq_ckpt8_store(code, rows, cols, ld, _ptr(x), _ptr(ck.codes), _ptr(ck.exponents), dev.index,
-                                          _stream(dev)))
+    _launch("dwbnq_ckpt8_store", dev, code, rows, cols, ld, x.data_ptr(), ck.codes.data_ptr(), ck.exponents.data_ptr())
     return ck
 
 
@@ -434,9 +463,7 @@ def restore_code8(ck, dtype=None, out=None):
     code = _few_bits_code(y.dtype)
     dev = _one_device(ck.codes, ck.exponents, y)
     rows, cols, ld = _rows_view(y, "out")
-    with torch.cuda.device(dev):
-        L.check(L.lib().dwbnq_ckpt8_load(code, rows, cols, _ptr(ck.codes), _ptr(ck.exponents), ld, _ptr(y), dev.index,
-                                         _stream(dev)))
+    _launch("dwbnq_ckpt8_load", dev, code, rows, cols, ck.codes.data_ptr(), ck.exponents.data_ptr(), ld, y.data_ptr())
     return y
 
 
@@ -446,14 +473,16 @@ def glu(gate, up, act="silu", checkpoint=False, out=None):
     code = _few_bits_code(gate.dtype)
     _like(up, "up", gate.shape, gate.dtype, gate.device)
     y = _like(out, "out", gate.shape, gate.dtype, gate.device)
-    cks = [Code8Checkpoint.empty(gate.shape, gate.dtype, gate.device) for _ in range(2)] if checkpoint else []
     dev = _one_device(gate, up, y)
     (rows, cols, ldg), (_, _, ldu), (_, _, ldy) = _rows_view(gate, "gate"), _rows_view(up, "up"), _rows_view(y, "out")
-    ptrs = [p for ck in cks for p in (_ptr(ck.codes), _ptr(ck.exponents))] or [None] * 4
-    with torch.cuda.device(dev):
-        L.check(L.lib().dwbnq_glu_fwd(code, _GLU_ACTS[act], rows, cols, ldg, _ptr(gate), ldu, _ptr(up), ldy, _ptr(y), *ptrs,
-                                      dev.index, _stream(dev)))
-    return (y, cks[0], cks[1]) if checkpoint else y
+    if not checkpoint:
+        _launch("dwbnq_glu_fwd", dev, code, _GLU_ACTS[act], rows, cols, ldg, gate.data_ptr(), ldu, up.data_ptr(), ldy,
+                y.data_ptr(), None, None, None, None)
+        return y
+    cg, cu = (Code8Checkpoint.empty(gate.shape, gate.dtype, dev) for _ in range(2))
+    _launch("dwbnq_glu_fwd", dev, code, _GLU_ACTS[act], rows, cols, ldg, gate.data_ptr(), ldu, up.data_ptr(), ldy, y.data_ptr(),
+            cg.codes.data_ptr(), cg.exponents.data_ptr(), cu.codes.data_ptr(), cu.exponents.data_ptr())
+    return y, cg, cu
 
 
 def glu_backward(ck_gate, ck_up, dy, act="silu", product=False, dgate=None, dup=None, need=(True, True),
@@ -461,29 +490,31 @@ def glu_backward(ck_gate, ck_up, dy, act="silu", product=False, dgate=None, dup=
     """Gradients of glu from the checkpoints of its inputs: (dgate, dup), None where ``need`` is False; with
     ``product`` also the checkpoint of act(gate) * up, the input of the layer behind. ``accum[i]`` adds onto
     the given tensor. dgate / dup may be views with a row stride, and either may be ``dy`` itself."""
-    if ck_gate.shape != ck_up.shape or ck_gate.dtype != ck_up.dtype:
-        raise ValueError("the checkpoints of gate and up must have one shape and type")
-    if any(a and n and t is None for a, n, t in zip(accum, need, (dgate, dup))):
-        raise ValueError("accumulating needs the tensor to accumulate onto")
     shape, dtype = ck_gate.shape, ck_gate.dtype
+    if ck_up.shape != shape or ck_up.dtype != dtype:
+        raise ValueError("the checkpoints of gate and up must have one shape and type")
+    if (accum[0] and need[0] and dgate is None) or (accum[1] and need[1] and dup is None):
+        raise ValueError("accumulating needs the tensor to accumulate onto")
     code = _few_bits_code(dtype)
-    device = ck_gate.codes.device
     if dy is None and (need[0] or need[1]):
         raise ValueError("dy is needed for dgate and dup")
+    device = ck_gate.codes.device
+    cols = ck_gate.cols
+    ldd = ldg = ldu = cols
     if dy is not None:
-        _like(dy, "dy", shape, dtype, device)
+        ldd = _rows_view(_like(dy, "dy", shape, dtype, device), "dy")[2]
     dgate = _like(dgate, "dgate", shape, dtype, device) if need[0] else None
     dup = _like(dup, "dup", shape, dtype, device) if need[1] else None
-    ck = Code8Checkpoint.empty(shape, dtype, device) if product else None
+    if dgate is not None:
+        ldg = _rows_view(dgate, "dgate")[2]
+    if dup is not None:
+        ldu = _rows_view(dup, "dup")[2]
     dev = _one_device(ck_gate.codes, ck_gate.exponents, ck_up.codes, ck_up.exponents, dy, dgate, dup)
-    rows, cols = ck_gate.rows, ck_gate.cols
-    ld = [_rows_view(t, n)[2] if t is not None else cols for t, n in ((dy, "dy"), (dgate, "dgate"), (dup, "dup"))]
+    ck = Code8Checkpoint.empty(shape, dtype, dev) if product else None
     mask = (1 if accum[0] else 0) | (2 if accum[1] else 0)
-    with torch.cuda.device(dev):
-        L.check(L.lib().dwbnq_glu_bwd_ckpt8(code, _GLU_ACTS[act], rows, cols, _ptr(ck_gate.codes), _ptr(ck_gate.exponents),
-                                            _ptr(ck_up.codes), _ptr(ck_up.exponents), ld[0], _ptr(dy), ld[1], _ptr(dgate),
-                                            ld[2], _ptr(dup), _ptr(ck.codes) if ck else None,
-                                            _ptr(ck.exponents) if ck else None, mask, dev.index, _stream(dev)))
+    _launch("dwbnq_glu_bwd_ckpt8", dev, code, _GLU_ACTS[act], ck_gate.rows, cols, ck_gate.codes.data_ptr(),
+            ck_gate.exponents.data_ptr(), ck_up.codes.data_ptr(), ck_up.exponents.data_ptr(), ldd, _addr(dy), ldg, _addr(dgate),
+            ldu, _addr(dup), ck.codes.data_ptr() if product else None, ck.exponents.data_ptr() if product else None, mask)
     return (dgate, dup, ck) if product else (dgate, dup)
 
 
@@ -513,13 +544,12 @@ def affine_weight_backward(ck_x, dy, dw=None, db=None, need=(True, True), accum=
     dev = _one_device(dy, ck_x.codes, ck_x.exponents, dw, db, ws)
     d = L.AffineDesc(dtype=code, dw_dtype=_few_bits_code(dtype), rows=rows, c_in=c_in, c_out=c_out, ld_dy=ld)
     mask = (2 if accum[0] else 0) | (4 if accum[1] else 0)
-    with torch.cuda.device(dev):
-        if ws is None:
-            ws = affine_workspace(d, dev)
-        elif ws.numel() * ws.element_size() < int(L.lib().dwbnq_affine_bwd_workspace_bytes(ctypes.byref(d))):
-            raise ValueError("ws is smaller than dwbnq_affine_bwd_workspace_bytes asks for")
-        L.check(L.lib().dwbnq_affine_bwd_ckpt8(ctypes.byref(d), _ptr(ck_x.codes), _ptr(ck_x.exponents), _ptr(dy), _ptr(dw),
-                                               _ptr(db), mask, _ptr(ws), dev.index, _stream(dev)))
+    if ws is None:
+        ws = affine_workspace(d, dev)
+    elif ws.numel() * ws.element_size() < int(L.lib().dwbnq_affine_bwd_workspace_bytes(ctypes.byref(d))):
+        raise ValueError("ws is smaller than dwbnq_affine_bwd_workspace_bytes asks for")
+    _launch("dwbnq_affine_bwd_ckpt8", dev, ctypes.byref(d), ck_x.codes.data_ptr(), ck_x.exponents.data_ptr(), dy.data_ptr(),
+            _addr(dw), _addr(db), mask, ws.data_ptr())
     return dw, db
 
 
@@ -528,10 +558,12 @@ class W4Weight:
 
     def __init__(self, packed, c_out, c_in, group, dtype, has_zeros):
         self.packed, self.c_out, self.c_in, self.group, self.dtype, self.has_zeros = packed, c_out, c_in, group, dtype, has_zeros
+        self._desc = L.W4Desc(dtype=_few_bits_code(dtype), group=group, c_in=c_in, c_out=c_out, has_zeros=int(has_zeros))
+        self._ref = ctypes.byref(self._desc)
 
     def desc(self):
-        return L.W4Desc(dtype=_few_bits_code(self.dtype), group=self.group, c_in=self.c_in, c_out=self.c_out,
-                        has_zeros=int(self.has_zeros))
+        """The layer's dwbnq_w4_desc, by reference."""
+        return self._ref
 
 
 def quantize_w4(w, group=128):
@@ -544,9 +576,7 @@ def quantize_w4(w, group=128):
     c_out, c_in, ld = _rows_view(w, "w")
     codes = torch.empty((c_out, c_in), dtype=torch.uint8, device=dev)
     scales = torch.empty((c_out, (c_in + group - 1) // group), dtype=w.dtype, device=dev)
-    with torch.cuda.device(dev):
-        L.check(L.lib().dwbnq_w4_quantize(code, c_out, c_in, group, ld, _ptr(w), _ptr(codes), _ptr(scales), dev.index,
-                                          _stream(dev)))
+    _launch("dwbnq_w4_quantize", dev, code, c_out, c_in, group, ld, _addr(w), _addr(codes), _addr(scales))
     return codes, scales
 
 
@@ -565,10 +595,8 @@ def pack_w4(codes, scales, zeros=None, group=128):
         raise ValueError("codes, scales and zeros must be contiguous")
     w4 = W4Weight(None, c_out, c_in, int(group), scales.dtype, zeros is not None)
     d = w4.desc()
-    with torch.cuda.device(dev):
-        w4.packed = torch.empty(int(L.lib().dwbnq_w4_packed_bytes(ctypes.byref(d))), dtype=torch.uint8, device=dev)
-        L.check(L.lib().dwbnq_w4_pack(ctypes.byref(d), _ptr(codes), _ptr(scales), _ptr(zeros), _ptr(w4.packed), dev.index,
-                                      _stream(dev)))
+    w4.packed = torch.empty(int(L.lib().dwbnq_w4_packed_bytes(d)), dtype=torch.uint8, device=dev)
+    _launch("dwbnq_w4_pack", dev, d, codes.data_ptr(), scales.data_ptr(), _addr(zeros), w4.packed.data_ptr())
     return w4
 
 
@@ -583,11 +611,8 @@ def affine_w4(x, w4, b=None, out=None):
     if b is not None and not _like(b, "b", (w4.c_out,), x.dtype, x.device).is_contiguous():
         raise ValueError("b must be contiguous")
     dev = _one_device(x, w4.packed, b, y)
-    _, _, ldy = _rows_view(y, "out")
-    d = w4.desc()
-    with torch.cuda.device(dev):
-        L.check(L.lib().dwbnq_w4_affine_fwd(ctypes.byref(d), rows, ldx, _ptr(x), _ptr(w4.packed), _ptr(b), ldy, _ptr(y),
-                                            dev.index, _stream(dev)))
+    _launch("dwbnq_w4_affine_fwd", dev, w4.desc(), rows, ldx, x.data_ptr(), w4.packed.data_ptr(), _addr(b),
+            _rows_view(y, "out")[2], y.data_ptr())
     return y
 
 
