@@ -17,7 +17,9 @@ constexpr int kThreads = 256;
 // 2 + 1.2 |g| of them): the result keeps 8 or 11 bits.
 template <typename T> __device__ __forceinline__ float glu_sigmoid(float g) {
   if (sizeof(T) == 4) return __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-g)));
-  return __fdividef(1.0f, __fadd_rn(1.0f, __expf(-g)));
+  float s;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(__fadd_rn(1.0f, __expf(-g))));
+  return s;
 }
 template <typename T, int ACT>
 __device__ __forceinline__ float act_value(float g) {
