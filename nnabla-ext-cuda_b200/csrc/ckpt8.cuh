@@ -46,12 +46,13 @@ __device__ __forceinline__ float ck_step(unsigned int b) {
 }
 // ---- eight consecutive values of a row: what a lane works on; four lanes share a group -----------------------
 
-// How a row of a tensor may be accessed: 16-byte vectors, 4-byte words (two 16-bit values, one fp32), or single values. The
-// same for every row, from the tensor's address and row stride.
-enum OctetAccess : int { OCTET_VALUE = 0, OCTET_WORD = 1, OCTET_VECTOR = 2 };
-inline int octet_access(const void *p, long long ld, int bytes) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * bytes);
-  return a % 16 == 0 ? OCTET_VECTOR : a % 4 == 0 ? OCTET_WORD : OCTET_VALUE;
+// Rows that all start on a 16-byte boundary are accessed in 16-byte vectors. Others value by value, but so that the lanes of a warp
+// touch consecutive values: the warp's 256 values change places through 1 KB of shared memory of its own (`stage`). Lane for lane
+// every instruction would touch 32 lines, and L2 saw every sector eight times (float32 [4099, 5003] restored: 72 us).
+// Every lane of the warp calls load and store, those past the end with n <= 0. A kernel is compiled for either way, as both in one
+// cost the first one's registers (a quarter of its speed).
+inline bool octet_vectors(const void *p, long long ld, int bytes) {
+  return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * bytes)) % 16) == 0;
 }
 // Two values of a 16-bit type in one word, to and from fp32.
 __device__ __forceinline__ void unpack_pair(const __nv_bfloat16 *, unsigned int w, float &lo, float &hi) {
@@ -72,52 +73,79 @@ __device__ __forceinline__ unsigned int pack_pair(const __half *, float lo, floa
   return *reinterpret_cast<const unsigned int *>(&r);
 }
 
-template <typename T> struct Octet {
+template <typename T, bool VECTORS> struct Octet {
   static constexpr int WORDS = 8 * (int)sizeof(T) / 4;
   // n: values that exist (the rest are 0); p is not followed for n <= 0
-  static __device__ __forceinline__ void load(const T *p, long long n, int access, float *v) {
-    unsigned int w[WORDS];
-    if (n >= 8 && access == OCTET_VECTOR) {
+  static __device__ __forceinline__ void load(const T *p, long long n, float *stage, float *v) {
+    if constexpr (VECTORS) {
+      unsigned int w[WORDS];
+      if (n >= 8) {
 #pragma unroll
-      for (int k = 0; k < WORDS / 4; ++k) {
-        const uint4 q = __ldcs(reinterpret_cast<const uint4 *>(p) + k);
-        w[4 * k] = q.x; w[4 * k + 1] = q.y; w[4 * k + 2] = q.z; w[4 * k + 3] = q.w;
+        for (int k = 0; k < WORDS / 4; ++k) {
+          const uint4 q = __ldcs(reinterpret_cast<const uint4 *>(p) + k);
+          w[4 * k] = q.x; w[4 * k + 1] = q.y; w[4 * k + 2] = q.z; w[4 * k + 3] = q.w;
+        }
+      } else {
+        T e[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) e[k] = k < n ? p[k] : Elem<T>::from_f32(0.0f);
+        memcpy(w, e, sizeof(w));
       }
-    } else if (n >= 8 && access == OCTET_WORD) {
 #pragma unroll
-      for (int k = 0; k < WORDS; ++k) w[k] = __ldg(reinterpret_cast<const unsigned int *>(p) + k);
+      for (int k = 0; k < WORDS; ++k) {
+        if constexpr (sizeof(T) == 4) v[k] = __uint_as_float(w[k]);
+        else unpack_pair(p, w[k], v[2 * k], v[2 * k + 1]);
+      }
     } else {
-      T e[8];
+      const int lane = threadIdx.x & 31, have = n < 8 ? (int)n : 8;
+      float t[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) e[k] = k < n ? p[k] : Elem<T>::from_f32(0.0f);
-      memcpy(w, e, sizeof(w));
-    }
+      for (int k = 0; k < 8; ++k) {  // value lane % 8 of lane 4 k + lane / 8
+        const int from = 4 * k + (lane >> 3);
+        const T *q = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), from));
+        const int m = __shfl_sync(0xffffffffu, have, from);
+        t[k] = (lane & 7) < m ? Elem<T>::to_f32(q[lane & 7]) : 0.0f;
+      }
 #pragma unroll
-    for (int k = 0; k < WORDS; ++k) {
-      if constexpr (sizeof(T) == 4) v[k] = __uint_as_float(w[k]);
-      else unpack_pair(p, w[k], v[2 * k], v[2 * k + 1]);
+      for (int k = 0; k < 8; ++k) stage[32 * k + lane] = t[k];
+      __syncwarp();
+      const float4 lo = reinterpret_cast<const float4 *>(stage)[2 * lane], hi = reinterpret_cast<const float4 *>(stage)[2 * lane + 1];
+      __syncwarp();
+      v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
     }
   }
-  static __device__ __forceinline__ void store(T *p, long long n, int access, const float *v) {
-    unsigned int w[WORDS];
+  static __device__ __forceinline__ void store(T *p, long long n, float *stage, const float *v) {
+    if constexpr (VECTORS) {
+      unsigned int w[WORDS];
 #pragma unroll
-    for (int k = 0; k < WORDS; ++k) {
-      if constexpr (sizeof(T) == 4) w[k] = __float_as_uint(v[k]);
-      else w[k] = pack_pair(p, v[2 * k], v[2 * k + 1]);
-    }
-    if (n >= 8 && access == OCTET_VECTOR) {
+      for (int k = 0; k < WORDS; ++k) {
+        if constexpr (sizeof(T) == 4) w[k] = __float_as_uint(v[k]);
+        else w[k] = pack_pair(p, v[2 * k], v[2 * k + 1]);
+      }
+      if (n >= 8) {
 #pragma unroll
-      for (int k = 0; k < WORDS / 4; ++k)
-        __stcs(reinterpret_cast<uint4 *>(p) + k, make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]));
-    } else if (n >= 8 && access == OCTET_WORD) {
+        for (int k = 0; k < WORDS / 4; ++k)
+          __stcs(reinterpret_cast<uint4 *>(p) + k, make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]));
+      } else {
+        T e[8];
+        memcpy(e, w, sizeof(w));
 #pragma unroll
-      for (int k = 0; k < WORDS; ++k) reinterpret_cast<unsigned int *>(p)[k] = w[k];
+        for (int k = 0; k < 8; ++k)
+          if (k < n) p[k] = e[k];
+      }
     } else {
-      T e[8];
-      memcpy(e, w, sizeof(w));
+      const int lane = threadIdx.x & 31, have = n < 8 ? (int)n : 8;
+      reinterpret_cast<float4 *>(stage)[2 * lane] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4 *>(stage)[2 * lane + 1] = make_float4(v[4], v[5], v[6], v[7]);
+      __syncwarp();
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (k < n) p[k] = e[k];
+      for (int k = 0; k < 8; ++k) {
+        const int from = 4 * k + (lane >> 3);
+        T *q = reinterpret_cast<T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), from));
+        const int m = __shfl_sync(0xffffffffu, have, from);
+        if ((lane & 7) < m) q[lane & 7] = Elem<T>::from_f32(stage[32 * k + lane]);
+      }
+      __syncwarp();
     }
   }
 };
@@ -157,6 +185,14 @@ __device__ __forceinline__ void octet_next(OctetWalk &w) {
   w.col += w.col_step;
   if (w.col >= w.per_row) { w.col -= w.per_row; ++w.row; }
 }
+
+template <bool VECTORS> struct OctetStage {  // the shared memory of a warp's exchange; none for vectors
+  static __device__ __forceinline__ float *get() {
+    if constexpr (VECTORS) return nullptr;
+    __shared__ float4 stages[512];  // 256 threads
+    return reinterpret_cast<float *>(stages) + (threadIdx.x >> 5) * 256;
+  }
+};
 
 // Writes the checkpoint of a lane's eight values; the four lanes of a group work together (all lanes of the warp call it).
 __device__ __forceinline__ void ck_put(const float *v, bool in, long long octet, signed char *codes, unsigned char *exps) {
