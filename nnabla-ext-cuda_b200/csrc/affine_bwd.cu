@@ -159,6 +159,12 @@ template <int PARTS, int BN, int DY, int TBYTES> struct DwStage {
                        RAW = CODES + CHUNK * kTileI, BYTES = RAW + (DY == DY_RAW ? CHUNK * BN * TBYTES : 0), COUNT = 4 * BYTES + 2048 <= kSmemMax ? 4 : 2;
 };
 
+// pw_wait for a warp of a CTA that may be giving up: the flag is looked at only when the barrier is not ready.
+__device__ __forceinline__ bool dw_wait(unsigned long long *bar, unsigned int parity, volatile int *abort_v) {
+  if (__all_sync(0xffffffffu, pw_try_wait(bar, parity))) return true;
+  return pw_wait(bar, parity) && !*abort_v;
+}
+
 // T: type of dy; TW: type of dw (32 bits: sums in short runs); PARTS: bfloat16 parts of dy; BN: output channels per tile.
 template <typename T, typename TW, int PARTS, int DY, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -224,7 +230,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
       constexpr int COLS = DyBox<T>::COLS, MAXBOX = BN / COLS, DYAT = DY == DY_RAW ? S::RAW : XB;
       const int boxes = DY == DY_LOAD ? 0 : min(MAXBOX, (a.c_out - o0 + COLS - 1) / COLS);
       for (int c = c0; c < c1; ++c) {
-        if (!pw_wait(&empty[s], ph ^ 1u) || *abort_v) { ok = false; break; }
+        if (!dw_wait(&empty[s], ph ^ 1u, abort_v)) { ok = false; break; }
         if (elect_one()) {
           unsigned char *st = sm + s * STAGE;
           mbar_expect_tx(&full[s], (boxes + 1) * BOX);
@@ -263,7 +269,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
       int run = 0;
       for (int c = c0; c < c1; ++c) {
         // dy and the codes of the stage have landed when its converters have arrived: they waited for them
-        if ((run == 0 && !pw_wait(&acc_empty[b], aph ^ 1u)) || !pw_wait(&conv[s], ph) || *abort_v) { ok = false; break; }
+        if ((run == 0 && !dw_wait(&acc_empty[b], aph ^ 1u, abort_v)) || !dw_wait(&conv[s], ph, abort_v)) { ok = false; break; }
         tc_fence_after();
         const bool last = c == c1 - 1 || (KEEP32 && run == RUN - 1);
         const unsigned long long so = (unsigned long long)(s * STAGE) >> 4;
@@ -276,7 +282,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
             const unsigned long long dx = dx0 + so, dd = dd0 + so + (unsigned)(p * (DYB >> 4));
 #pragma unroll
             for (int j = 0; j < CHUNK / 16; ++j)  // a step is 16 rows of 128 bytes
-              if (j < steps) tc_mma_f16(d, dx + j * 128, dd + j * 128, idesc, run || j || p < PARTS - 1 ? 1u : 0u);
+              if (j == 0 || j < steps) tc_mma_f16(d, dx + j * 128, dd + j * 128, idesc, j || p < PARTS - 1 ? 1u : run ? 1u : 0u);
           }
           tc_commit(&empty[s]);
           if (last) tc_commit(&acc_full[b]);
@@ -338,7 +344,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
       const int c_now = c, o = tile / a.i_tiles * BN + l16 * 8;
       move(STAGES);
       exponents(ex_next);
-      if (!pw_wait(&full[g], ph) || *abort_v) { ok = false; break; }
+      if (!dw_wait(&full[g], ph, abort_v)) { ok = false; break; }
 #pragma unroll
       for (int p = 0; p < TOKENS / 2; ++p) {
         const unsigned int r = tok0 + 2 * p + hi;
@@ -404,7 +410,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
       };
       const int runs = KEEP32 ? (c1 - c0 + RUN - 1) / RUN : 1;
       for (int r = 0; ok && r < runs; ++r) {
-        if (!pw_wait(&acc_full[b], aph) || *abort_v) { ok = false; break; }
+        if (!dw_wait(&acc_full[b], aph, abort_v)) { ok = false; break; }
         tc_fence_after();
         const unsigned int taddr = tmem_base + ((unsigned)(quarter * 32) << 16) + b * BN + half * HALF;
 #pragma unroll 1
@@ -440,57 +446,93 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
   }
 }
 
-// dw of the tiles whose tokens were cut into `segs` parts: the parts added in order. CTA = tile x 16 of its columns.
+// dw of the tiles whose tokens were cut into `segs` parts: the parts added in order, eight of them in flight. CTA = tile x two of
+// its columns.
 template <typename TW>
-__global__ void __launch_bounds__(kTileI)
+__global__ void __launch_bounds__(2 * kTileI)
     affine_dw_join_kernel(const float *__restrict__ parts, int first_tile, int segs, int bn, int i_tiles, int c_in, int c_out,
                           TW *__restrict__ dw, int accum) {
   pdl_launch_dependents();
   pdl_wait_for_predecessor();
-  const int tile = first_tile + blockIdx.x, ot = tile / i_tiles, i = (tile - ot * i_tiles) * kTileI + threadIdx.x;
-  if (i >= c_in) return;
-  const float *p = parts + ((long long)blockIdx.x * segs * bn + blockIdx.y * 16) * kTileI + threadIdx.x;
-#pragma unroll 4
-  for (int n = 0; n < 16; ++n) {
-    const int o = ot * bn + blockIdx.y * 16 + n;
-    if (o >= c_out) return;
-    float s = p[n * kTileI];
-    for (int k = 1; k < segs; ++k) s = __fadd_rn(s, p[((long long)k * bn + n) * kTileI]);
-    TW *q = dw + (long long)o * c_in + i;
-    *q = Elem<TW>::from_f32(accum ? __fadd_rn(Elem<TW>::to_f32(*q), s) : s);
+  const int tile = first_tile + blockIdx.x, ot = tile / i_tiles, il = threadIdx.x % kTileI, n = blockIdx.y * 2 + threadIdx.x / kTileI;
+  const int i = (tile - ot * i_tiles) * kTileI + il, o = ot * bn + n;
+  if (i >= c_in || o >= c_out) return;
+  const float *p = parts + ((long long)blockIdx.x * segs * bn + n) * kTileI + il;
+  const long long step = (long long)bn * kTileI;
+  float s = 0.0f;
+  for (int k = 0; k < segs; k += 8) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = k + j < segs ? p[(k + j) * step] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = __fadd_rn(s, v[j]);
   }
+  TW *q = dw + (long long)o * c_in + i;
+  *q = Elem<TW>::from_f32(accum ? __fadd_rn(Elem<TW>::to_f32(*q), s) : s);
 }
 
-// ---- bias gradient: CTA (32 channels, slice of the rows), warp w the rows w, w + 8, ...; then the slices in order ----
+// ---- bias gradient: CTA (64 channels, slice of the rows), a lane two channels, warp w the rows w, w + 8, ..., four of them in
+// flight; then the slices in order. PAIRS: the two channels of a row are one aligned load ----
 constexpr int kDbSlices = 64;
 
-template <typename T>
+template <typename T, bool PAIRS>
 __global__ void __launch_bounds__(256)
     affine_db_kernel(long long rows, int c_out, const T *__restrict__ dy, long long ld, float *__restrict__ part) {
   pdl_launch_dependents();
   pdl_wait_for_predecessor();
-  __shared__ float sums[8][32];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, o = blockIdx.x * 32 + lane;
+  __shared__ float sums[8][64];
+  struct __align__(2 * sizeof(T)) Pair { T a, b; };
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, o = blockIdx.x * 64 + 2 * lane;
   const long long r0 = rows * blockIdx.y / gridDim.y, r1 = rows * (blockIdx.y + 1) / gridDim.y;
-  float s = 0.0f;
-  if (o < c_out)
-    for (long long t = r0 + w; t < r1; t += 8) s = __fadd_rn(s, Elem<T>::to_f32(dy[t * ld + o]));
-  sums[w][lane] = s;
-  __syncthreads();
-  if (w || o >= c_out) return;
+  const bool a_ok = o < c_out, b_ok = o + 1 < c_out;
+  float s0 = 0.0f, s1 = 0.0f;
+  for (long long t = r0 + w; t < r1; t += 32) {
+    float v[4][2];
 #pragma unroll
-  for (int i = 1; i < 8; ++i) s = __fadd_rn(s, sums[i][lane]);
-  part[(long long)blockIdx.y * c_out + o] = s;
+    for (int j = 0; j < 4; ++j) {
+      const T *q = dy + (t + 8 * j) * ld + o;
+      const bool in = t + 8 * j < r1;
+      if (PAIRS && b_ok) {
+        Pair e = {Elem<T>::from_f32(0.0f), Elem<T>::from_f32(0.0f)};
+        if (in) e = *reinterpret_cast<const Pair *>(q);
+        v[j][0] = Elem<T>::to_f32(e.a);
+        v[j][1] = Elem<T>::to_f32(e.b);
+      } else {
+        v[j][0] = in && a_ok ? Elem<T>::to_f32(q[0]) : 0.0f;
+        v[j][1] = in && b_ok ? Elem<T>::to_f32(q[1]) : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      s0 = __fadd_rn(s0, v[j][0]);
+      s1 = __fadd_rn(s1, v[j][1]);
+    }
+  }
+  sums[w][2 * lane] = s0;
+  sums[w][2 * lane + 1] = s1;
+  __syncthreads();
+  const int c = threadIdx.x;
+  if (c >= 64 || blockIdx.x * 64 + c >= c_out) return;
+  float s = sums[0][c];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) s = __fadd_rn(s, sums[i][c]);
+  part[(long long)blockIdx.y * c_out + blockIdx.x * 64 + c] = s;
 }
 template <typename TW>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(64)
     affine_db_join_kernel(const float *__restrict__ part, int slices, int c_out, TW *__restrict__ db, int accum) {
   pdl_launch_dependents();
   pdl_wait_for_predecessor();
-  const int o = blockIdx.x * 256 + threadIdx.x;
+  const int o = blockIdx.x * 64 + threadIdx.x;
   if (o >= c_out) return;
   float s = 0.0f;
-  for (int i = 0; i < slices; ++i) s = __fadd_rn(s, part[(long long)i * c_out + o]);
+  for (int i = 0; i < slices; i += 16) {
+    float v[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = i + j < slices ? part[(long long)(i + j) * c_out + o] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s = __fadd_rn(s, v[j]);
+  }
   db[o] = Elem<TW>::from_f32(accum ? __fadd_rn(Elem<TW>::to_f32(db[o]), s) : s);
 }
 
@@ -558,6 +600,14 @@ int launch_dw(const CUtensorMap &tm, const CUtensorMap &tc, const DwArgs &a, cud
   return e == cudaSuccess ? DWBNQ_OK : fail_cuda(e, "affine_dw_kernel launch");
 }
 
+template <typename T>
+cudaError_t launch_db(const dwbnq_affine_desc &d, const T *dy, int slices, float *parts, cudaStream_t stream) {
+  const dim3 grid((unsigned)((d.c_out + 63) / 64), (unsigned)slices);
+  const bool pairs = reinterpret_cast<uintptr_t>(dy) % (2 * sizeof(T)) == 0 && d.ld_dy % 2 == 0;
+  return pairs ? launch_pdl(affine_db_kernel<T, true>, grid, dim3(256), 0, stream, (long long)d.rows, d.c_out, dy, (long long)d.ld_dy, parts)
+               : launch_pdl(affine_db_kernel<T, false>, grid, dim3(256), 0, stream, (long long)d.rows, d.c_out, dy, (long long)d.ld_dy, parts);
+}
+
 template <typename TW>
 int run_t(const dwbnq_affine_desc &d, const void *codes, const void *exps, const void *dy, void *dw, void *db, int accum_mask,
           void *workspace, int dev, cudaStream_t stream) {
@@ -622,23 +672,19 @@ int run_t(const dwbnq_affine_desc &d, const void *codes, const void *exps, const
     }
     if (st != DWBNQ_OK) return st;
     if (p.segs > 1) {
-      const dim3 grid((unsigned)((p.units - p.full) / p.segs), (unsigned)(p.bn / 16));
-      e = launch_pdl(affine_dw_join_kernel<TW>, grid, dim3(kTileI), 0, stream, (const float *)parts, p.full, p.segs, p.bn, p.i_tiles,
+      const dim3 grid((unsigned)((p.units - p.full) / p.segs), (unsigned)(p.bn / 2));
+      e = launch_pdl(affine_dw_join_kernel<TW>, grid, dim3(2 * kTileI), 0, stream, (const float *)parts, p.full, p.segs, p.bn, p.i_tiles,
                      d.c_in, d.c_out, static_cast<TW *>(dw), (accum_mask >> 1) & 1);
       if (e != cudaSuccess) return fail_cuda(e, "affine_dw_join_kernel launch");
     }
   }
   if (db) {
     const int slices = (int)(d.rows < 32 ? 1 : d.rows / 32 < kDbSlices ? d.rows / 32 : kDbSlices);
-    const dim3 grid((unsigned)((d.c_out + 31) / 32), (unsigned)slices);
-    if (d.dtype == DWBNQ_F32)
-      e = launch_pdl(affine_db_kernel<float>, grid, dim3(256), 0, stream, (long long)d.rows, d.c_out, static_cast<const float *>(dy), (long long)d.ld_dy, dbp);
-    else if (d.dtype == DWBNQ_F16)
-      e = launch_pdl(affine_db_kernel<__half>, grid, dim3(256), 0, stream, (long long)d.rows, d.c_out, static_cast<const __half *>(dy), (long long)d.ld_dy, dbp);
-    else
-      e = launch_pdl(affine_db_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, (long long)d.rows, d.c_out, static_cast<const __nv_bfloat16 *>(dy), (long long)d.ld_dy, dbp);
+    if (d.dtype == DWBNQ_F32) e = launch_db(d, static_cast<const float *>(dy), slices, dbp, stream);
+    else if (d.dtype == DWBNQ_F16) e = launch_db(d, static_cast<const __half *>(dy), slices, dbp, stream);
+    else e = launch_db(d, static_cast<const __nv_bfloat16 *>(dy), slices, dbp, stream);
     if (e != cudaSuccess) return fail_cuda(e, "affine_db_kernel launch");
-    e = launch_pdl(affine_db_join_kernel<TW>, dim3((unsigned)((d.c_out + 255) / 256)), dim3(256), 0, stream, (const float *)dbp, slices, d.c_out,
+    e = launch_pdl(affine_db_join_kernel<TW>, dim3((unsigned)((d.c_out + 63) / 64)), dim3(64), 0, stream, (const float *)dbp, slices, d.c_out,
                    static_cast<TW *>(db), (accum_mask >> 2) & 1);
     if (e != cudaSuccess) return fail_cuda(e, "affine_db_join_kernel launch");
   }
