@@ -471,9 +471,9 @@ __global__ void __launch_bounds__(2 * kTileI)
   *q = Elem<TW>::from_f32(accum ? __fadd_rn(Elem<TW>::to_f32(*q), s) : s);
 }
 
-// ---- bias gradient: CTA (64 channels, slice of the rows), a lane two channels, warp w the rows w, w + 8, ..., four of them in
-// flight; then the slices in order. PAIRS: the two channels of a row are one aligned load ----
-constexpr int kDbSlices = 64;
+// ---- bias gradient: CTA (64 channels, slice of the rows), a lane two channels, warp w the rows w, w + 8, ..., eight of them in
+// flight; then the slices in order, a quarter of them per thread and the quarters in order. PAIRS: the two channels of a row are one aligned load ----
+constexpr int kDbMaxSlices = 256;
 
 template <typename T, bool PAIRS>
 __global__ void __launch_bounds__(256)
@@ -486,10 +486,10 @@ __global__ void __launch_bounds__(256)
   const long long r0 = rows * blockIdx.y / gridDim.y, r1 = rows * (blockIdx.y + 1) / gridDim.y;
   const bool a_ok = o < c_out, b_ok = o + 1 < c_out;
   float s0 = 0.0f, s1 = 0.0f;
-  for (long long t = r0 + w; t < r1; t += 32) {
-    float v[4][2];
+  for (long long t = r0 + w; t < r1; t += 64) {
+    float v[8][2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 8; ++j) {
       const T *q = dy + (t + 8 * j) * ld + o;
       const bool in = t + 8 * j < r1;
       if (PAIRS && b_ok) {
@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(256)
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 8; ++j) {
       s0 = __fadd_rn(s0, v[j][0]);
       s1 = __fadd_rn(s1, v[j][1]);
     }
@@ -519,20 +519,24 @@ __global__ void __launch_bounds__(256)
   part[(long long)blockIdx.y * c_out + blockIdx.x * 64 + c] = s;
 }
 template <typename TW>
-__global__ void __launch_bounds__(64)
+__global__ void __launch_bounds__(256)
     affine_db_join_kernel(const float *__restrict__ part, int slices, int c_out, TW *__restrict__ db, int accum) {
   pdl_launch_dependents();
   pdl_wait_for_predecessor();
-  const int o = blockIdx.x * 64 + threadIdx.x;
-  if (o >= c_out) return;
+  __shared__ float sums[4][64];
+  const int c = threadIdx.x & 63, q = threadIdx.x >> 6, o = blockIdx.x * 64 + c;
   float s = 0.0f;
-  for (int i = 0; i < slices; i += 16) {
+  for (int i = slices * q / 4, end = slices * (q + 1) / 4; i < end; i += 16) {
     float v[16];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = i + j < slices ? part[(long long)(i + j) * c_out + o] : 0.0f;
+    for (int j = 0; j < 16; ++j) v[j] = i + j < end && o < c_out ? part[(long long)(i + j) * c_out + o] : 0.0f;
 #pragma unroll
     for (int j = 0; j < 16; ++j) s = __fadd_rn(s, v[j]);
   }
+  sums[q][c] = s;
+  __syncthreads();
+  if (q || o >= c_out) return;
+  s = __fadd_rn(__fadd_rn(s, sums[1][c]), __fadd_rn(sums[2][c], sums[3][c]));
   db[o] = Elem<TW>::from_f32(accum ? __fadd_rn(Elem<TW>::to_f32(db[o]), s) : s);
 }
 
@@ -543,6 +547,13 @@ struct DwPlan {
   size_t parts_bytes, bytes;
 };
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Slices of the rows for the bias gradient: eight CTAs per SM, at least 64 rows each.
+int db_slices(const dwbnq_affine_desc &d) {
+  const long long ctas = (d.c_out + 63) / 64, by_rows = d.rows / 64, want = 8 * kPlanSms / (ctas > 0 ? ctas : 1);
+  const long long s = by_rows < want ? by_rows : want;
+  return (int)(s < 1 ? 1 : s > kDbMaxSlices ? kDbMaxSlices : s);
+}
 
 // `wide`: tiles of 256 output channels. Whole waves of kPlanSms tiles are walked uncut; the R tiles left over are cut into
 // the number of parts that costs least, in chunks on the busiest SM: ceil(R s / SMs) parts of ceil(chunks / s)
@@ -566,7 +577,7 @@ DwPlan dw_plan(const dwbnq_affine_desc &d, bool wide) {
   if (p.segs == 1) p.full = (int)tiles;
   p.units = p.segs == 1 ? (int)tiles : p.full + rest * p.segs;
   p.parts_bytes = p.segs == 1 ? 0 : up256((size_t)rest * p.segs * p.bn * kTileI * 4);
-  p.bytes = 256 + p.parts_bytes + up256((size_t)kDbSlices * d.c_out * 4);
+  p.bytes = 256 + p.parts_bytes + up256((size_t)db_slices(d) * d.c_out * 4);
   return p;
 }
 bool dw_wide(const dwbnq_affine_desc &d) { return d.dtype == DWBNQ_BF16; }
@@ -679,12 +690,12 @@ int run_t(const dwbnq_affine_desc &d, const void *codes, const void *exps, const
     }
   }
   if (db) {
-    const int slices = (int)(d.rows < 32 ? 1 : d.rows / 32 < kDbSlices ? d.rows / 32 : kDbSlices);
+    const int slices = db_slices(d);
     if (d.dtype == DWBNQ_F32) e = launch_db(d, static_cast<const float *>(dy), slices, dbp, stream);
     else if (d.dtype == DWBNQ_F16) e = launch_db(d, static_cast<const __half *>(dy), slices, dbp, stream);
     else e = launch_db(d, static_cast<const __nv_bfloat16 *>(dy), slices, dbp, stream);
     if (e != cudaSuccess) return fail_cuda(e, "affine_db_kernel launch");
-    e = launch_pdl(affine_db_join_kernel<TW>, dim3((unsigned)((d.c_out + 63) / 64)), dim3(64), 0, stream, (const float *)dbp, slices, d.c_out,
+    e = launch_pdl(affine_db_join_kernel<TW>, dim3((unsigned)((d.c_out + 63) / 64)), dim3(256), 0, stream, (const float *)dbp, slices, d.c_out,
                    static_cast<TW *>(db), (accum_mask >> 2) & 1);
     if (e != cudaSuccess) return fail_cuda(e, "affine_db_join_kernel launch");
   }
