@@ -353,7 +353,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
         *reinterpret_cast<uint4 *>(st + box + r * 128 + (((l16 & 7) ^ (r & 7)) << 4)) = dw_expand(code, e, magic);
       }
       if (DY != DY_TMA) {
-#pragma unroll 1
+#pragma unroll 4
         for (int p = 0; p < TOKENS / 2; ++p) {
           const unsigned int r = tok0 + 2 * p + hi;
           const long long t = (long long)c_now * CHUNK + r;
@@ -600,11 +600,12 @@ EncodeFn encode_fn() {
 }
 
 template <typename T, typename TW, int PARTS, int DY, int BN>
-int launch_dw(const CUtensorMap &tm, const CUtensorMap &tc, const DwArgs &a, cudaStream_t stream) {
+int launch_dw(const CUtensorMap &tm, const CUtensorMap &tc, const DwArgs &a, int dev, cudaStream_t stream) {
   using S = DwStage<PARTS, BN, DY, (int)sizeof(T)>;
   const int smem = S::COUNT * S::BYTES + 1024;
   auto kern = affine_dw_kernel<T, TW, PARTS, DY, BN>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<unsigned long long> allowed{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void *>(kern), smem, dev, allowed);
   if (e != cudaSuccess) return fail_cuda(e, "affine_dw_kernel attributes");
   const int sms = sm_count(-1);
   e = launch_pdl(kern, dim3((unsigned)(a.units < sms ? a.units : sms)), dim3(kThreads), (size_t)smem, stream, tm, tc, a);
@@ -669,17 +670,17 @@ int run_t(const dwbnq_affine_desc &d, const void *codes, const void *exps, const
     }
     if constexpr (sizeof(TW) == 4) {
       if (d.dtype == DWBNQ_F32)
-        st = tma ? launch_dw<float, TW, 3, DY_RAW, 128>(tm, tc, a, stream) : launch_dw<float, TW, 3, DY_LOAD, 128>(tm, tc, a, stream);
+        st = tma ? launch_dw<float, TW, 3, DY_RAW, 128>(tm, tc, a, dev, stream) : launch_dw<float, TW, 3, DY_LOAD, 128>(tm, tc, a, dev, stream);
       else if (d.dtype == DWBNQ_F16)
-        st = tma ? launch_dw<__half, TW, 2, DY_RAW, 128>(tm, tc, a, stream) : launch_dw<__half, TW, 2, DY_LOAD, 128>(tm, tc, a, stream);
+        st = tma ? launch_dw<__half, TW, 2, DY_RAW, 128>(tm, tc, a, dev, stream) : launch_dw<__half, TW, 2, DY_LOAD, 128>(tm, tc, a, dev, stream);
       else
-        st = tma ? launch_dw<__nv_bfloat16, TW, 1, DY_TMA, 256>(tm, tc, a, stream)
-                 : launch_dw<__nv_bfloat16, TW, 1, DY_LOAD, 128>(tm, tc, a, stream);
+        st = tma ? launch_dw<__nv_bfloat16, TW, 1, DY_TMA, 256>(tm, tc, a, dev, stream)
+                 : launch_dw<__nv_bfloat16, TW, 1, DY_LOAD, 128>(tm, tc, a, dev, stream);
     } else if constexpr (std::is_same<TW, __half>::value) {
-      st = tma ? launch_dw<__half, TW, 2, DY_RAW, 128>(tm, tc, a, stream) : launch_dw<__half, TW, 2, DY_LOAD, 128>(tm, tc, a, stream);
+      st = tma ? launch_dw<__half, TW, 2, DY_RAW, 128>(tm, tc, a, dev, stream) : launch_dw<__half, TW, 2, DY_LOAD, 128>(tm, tc, a, dev, stream);
     } else {
-      st = tma ? launch_dw<__nv_bfloat16, TW, 1, DY_TMA, 256>(tm, tc, a, stream)
-               : launch_dw<__nv_bfloat16, TW, 1, DY_LOAD, 128>(tm, tc, a, stream);
+      st = tma ? launch_dw<__nv_bfloat16, TW, 1, DY_TMA, 256>(tm, tc, a, dev, stream)
+               : launch_dw<__nv_bfloat16, TW, 1, DY_LOAD, 128>(tm, tc, a, dev, stream);
     }
     if (st != DWBNQ_OK) return st;
     if (p.segs > 1) {

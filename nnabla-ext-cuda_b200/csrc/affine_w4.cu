@@ -16,6 +16,7 @@ namespace dwbnq {
 namespace {
 
 constexpr int kPlanSms = 148;  // SMs of a B200
+constexpr int kSmemMax = 227 * 1024 - 1024;  // dynamic shared memory a CTA may ask for beside its static part
 constexpr int kTileO = 16, kTileI = 128, kTileBytes = kTileO * kTileI / 2;
 
 struct W4Layout {
@@ -216,6 +217,7 @@ struct W4Args {
   int ring;       // copies in flight per warp and tile
   int red_at, sums_at;  // where the sums lie in shared memory
   int vec;        // rows of x are 16-byte aligned
+  int device;
   int *flag;
 };
 
@@ -474,8 +476,10 @@ int affine_launch(W4Args a, int warps, int cluster, int ctas, cudaStream_t strea
   a.sums_at = a.red_at + 2 * warps * per_warp * (int)sizeof(float);
   const size_t smem = a.sums_at + (cluster > 1 ? 2 * sizeof(float) * (size_t)per_warp * cluster : 0);
   auto kern = w4_affine_kernel<T, G, NB, R, ZEROS>;
+  if (smem > (size_t)kSmemMax) return fail(DWBNQ_ERR_UNSUPPORTED, "w4: %zu bytes of shared memory", smem);
   if (smem > 40 * 1024) {  // above 48 KB with the static part
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<unsigned long long> allowed{0};
+    const cudaError_t e = allow_smem(reinterpret_cast<const void *>(kern), kSmemMax, a.device, allowed);
     if (e != cudaSuccess) return fail_cuda(e, "w4_affine_kernel attributes");
   }
   cudaLaunchConfig_t lc = {};
@@ -525,6 +529,7 @@ int affine_t(const dwbnq_w4_desc &d, long long rows, long long ld_x, const void 
   a.x = x; a.b = b; a.y = y;
   a.packed = static_cast<const unsigned char *>(packed);
   a.block = l.block;
+  a.device = dev;
   a.ld_x = ld_x; a.ld_y = ld_y;
   a.rows = (int)rows; a.c_in = d.c_in; a.c_out = d.c_out; a.i_tiles = (int)l.i_tiles; a.o_tiles = (int)l.o_tiles;
   a.vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_x * sizeof(T) % 16 == 0;

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <utility>
 
 #include "../../include/dwbnq.h"
@@ -41,6 +42,16 @@ cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t sme
   lc.attrs = attr;
   lc.numAttrs = pdl_enabled() ? 1 : 0;
   return cudaLaunchKernelEx(&lc, kern, std::forward<Args>(args)...);
+}
+
+// Lets a kernel have `bytes` of dynamic shared memory on `device`. Asked for once per kernel and device (`done`: one word of the
+// caller's per kernel, a bit per device): the driver call costs as much as a small launch.
+inline cudaError_t allow_smem(const void *kern, int bytes, int device, std::atomic<unsigned long long> &done) {
+  const unsigned long long bit = 1ull << (device & 63);
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && device < 64) done.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 // ---- fused / dw-conv family (fused.cu) --------------------------------------------------
