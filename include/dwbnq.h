@@ -406,12 +406,13 @@ int dwbnq_pwconv_plan(const dwbnq_pwconv_desc *desc, const void *x, const void *
  * [64, 128) (lower for magnitudes below 2^-120, where the step stays 2^-126). A group that holds
  * a NaN or an infinity has b = 255 and codes 0 and stands for NaN throughout. The arithmetic is
  * exact, so the result is the same bit for bit whoever computes it.
- *   codes: int8 [rows, 32 * ceil(cols / 32)], 16-byte aligned; codes past cols are written as 0
- *          (and what stands there is ignored by no reader: keep them 0);
+ *   codes: int8 [rows, 32 * ceil(cols / 32)], 16-byte aligned; codes past cols are written as 0;
  *   exps:  uint8 [rows, ceil(cols / 32)].
  * Row strides (ld_*) count elements, are at least cols, and may take any value and alignment;
  * strides that are multiples of 16 bytes on 16-byte aligned tensors are faster. rows, cols (c_in,
- * c_out) may be 0: then nothing is read, and gradients are those of an empty batch. */
+ * c_out) may be 0: then nothing is read, and gradients are those of an empty batch. Outputs must
+ * not overlap inputs unless an entry says so. Kernels that wait for copies do so for a bounded
+ * time; dwbnq_check_device_flag tells whether one ran out. */
 int dwbnq_ckpt8_store(int dtype, int64_t rows, int64_t cols, int64_t ld_x, const void *x, void *codes,
                       void *exps, int device, void *stream);
 /* y = the values the checkpoint stands for, rounded to dtype (exact for DWBNQ_F32 and DWBNQ_BF16). */

@@ -80,9 +80,9 @@ int check_dtype_few_bits(int dtype) {
     return fail(DWBNQ_ERR_INVALID_ARG, "dtype %d is none of DWBNQ_F32, DWBNQ_F16 and DWBNQ_BF16", dtype);
   return DWBNQ_OK;
 }
-constexpr int64_t kMaxSide = (int64_t)1 << 40;  // keeps rows * stride in 64 bits once the product is checked
+constexpr int64_t kMaxRows = (int64_t)1 << 40, kMaxCols = (int64_t)1 << 33;  // columns are counted in eights with 32 bits
 int check_matrix(const char *what, int64_t rows, int64_t cols, int64_t ld) {
-  if (rows < 0 || cols < 0 || rows > kMaxSide || cols > kMaxSide)
+  if (rows < 0 || cols < 0 || rows > kMaxRows || cols > kMaxCols)
     return fail(DWBNQ_ERR_INVALID_ARG, "%s: [%lld, %lld] is not a valid shape", what, (long long)rows, (long long)cols);
   if (ld < cols) return fail(DWBNQ_ERR_INVALID_ARG, "%s: row stride %lld below %lld columns", what, (long long)ld, (long long)cols);
   if (rows > 0 && ld > ((int64_t)1 << 60) / rows)
@@ -105,13 +105,15 @@ int check_glu_act(int act) {
     return fail(DWBNQ_ERR_INVALID_ARG, "activation %d is none of SILU, GELU and RELU", act);
   return DWBNQ_OK;
 }
+constexpr int64_t kMaxWeights = (int64_t)1 << 40;  // more than fits any memory; tiles of weights are counted with 32 bits
 int check_affine(const dwbnq_affine_desc *d) {
   if (!d) return fail(DWBNQ_ERR_INVALID_ARG, "affine desc is null");
   int st = check_dtype_few_bits(d->dtype);
   if (st != DWBNQ_OK) return st;
   if (d->dw_dtype != d->dtype && d->dw_dtype != DWBNQ_F32)
     return fail(DWBNQ_ERR_INVALID_ARG, "dw_dtype %d is neither the type of dy nor DWBNQ_F32", d->dw_dtype);
-  if (d->c_in < 0 || d->c_out < 0 || d->c_in > (1 << 24) || d->c_out > (1 << 24) || d->rows > ((int64_t)1 << 31) - 256)
+  if (d->c_in < 0 || d->c_out < 0 || d->c_in > (1 << 24) || d->c_out > (1 << 24) || (int64_t)d->c_in * d->c_out > kMaxWeights ||
+      d->rows > ((int64_t)1 << 31) - 256)
     return fail(DWBNQ_ERR_INVALID_ARG, "affine layer [%lld rows] %d -> %d is out of range", (long long)d->rows, d->c_in, d->c_out);
   return check_matrix("dy", d->rows, d->c_out, d->ld_dy);
 }
@@ -121,7 +123,7 @@ int check_w4(const dwbnq_w4_desc *d) {
   if (st != DWBNQ_OK) return st;
   if (d->group != 32 && d->group != 64 && d->group != 128)
     return fail(DWBNQ_ERR_UNSUPPORTED, "group of %d input channels: 32, 64 and 128 are supported", d->group);
-  if (d->c_in < 0 || d->c_out < 0 || d->c_in > (1 << 24) || d->c_out > (1 << 24))
+  if (d->c_in < 0 || d->c_out < 0 || d->c_in > (1 << 24) || d->c_out > (1 << 24) || (int64_t)d->c_in * d->c_out > kMaxWeights)
     return fail(DWBNQ_ERR_INVALID_ARG, "affine layer %d -> %d is out of range", d->c_in, d->c_out);
   return DWBNQ_OK;
 }

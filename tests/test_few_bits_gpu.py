@@ -523,3 +523,78 @@ def test_threads_share_nothing(cuda_device):
     [t.join() for t in threads]
     assert not errors
     assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
+# ---- sizes and places ---------------------------------------------------------------------------------------------
+
+def test_offsets_past_32_bits(cuda_device):
+    """Tensors of more than 2^31 elements: what lies at their far end is what the same rows give by themselves."""
+    rows, cols = 70001, 32768
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device=cuda_device)
+    tail = torch.randn(3, cols, generator=gen(1)).bfloat16().to(cuda_device)
+    x[-3:] = tail
+    ck, part = ops.checkpoint_code8(x), ops.checkpoint_code8(tail)
+    assert torch.equal(ck.codes[-3:], part.codes) and torch.equal(ck.exponents[-3:], part.exponents)
+    y = ops.restore_code8(ck, out=x)
+    assert torch.equal(y[-3:], ops.restore_code8(part)) and not y[:-3].any()
+    dy = torch.zeros(rows, 24, dtype=torch.bfloat16, device=cuda_device)
+    dy[-3:] = 1.0
+    dw, db = ops.affine_weight_backward(ck, dy, dtype=torch.float32)
+    want = ops.restore_code8(part, dtype=torch.float32).sum(0)
+    assert torch.allclose(dw, want.expand(24, cols), rtol=3 * 2.0 ** -23, atol=0) and (db == 3).all()
+    ops.check_device_flag()
+
+
+def test_w4_offsets_past_32_bits(cuda_device):
+    n, k = 65552, 65600
+    codes = torch.full((n, k), 8, dtype=torch.uint8, device=cuda_device)
+    codes[-5:] = torch.randint(0, 16, (5, k), generator=gen(2)).to(torch.uint8).to(cuda_device)
+    scales = torch.full((n, (k + 127) // 128), 0.5, dtype=torch.bfloat16, device=cuda_device)
+    w4 = ops.pack_w4(codes, scales, group=128)
+    assert w4.packed.numel() > 1 << 31
+    x = torch.randint(-1, 2, (2, k), generator=gen(3)).bfloat16().to(cuda_device)
+    y = ops.affine_w4(x, w4)
+    want = x.double() @ ((codes[-5:].double() - 8) * 0.5).T
+    assert torch.equal(y[:, -5:], want.bfloat16()) and not y[:, :-5].any()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_every_row_count(cuda_device, dt):
+    """Token counts around the chunk and run sizes of the weight gradient, and row counts of the 4-bit layer around its blocks."""
+    dtype = fb.TYPES[dt]
+    for rows in (2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257, 1023, 1025):
+        x, dy = dw_case(rows, 48, 40, dtype, rows, True)
+        dw, db = ops.affine_weight_backward(ops.checkpoint_code8(x.to(cuda_device)), dy.to(cuda_device), dtype=torch.float32)
+        assert torch.equal(dw.cpu(), (dy.double().T @ x.double()).float()) and torch.equal(db.cpu(), dy.double().sum(0).float())
+    x, codes, scales, zeros, _ = w4_case(35, 384, 40, 64, dtype, 5, True, True)
+    w4 = ops.pack_w4(*(t.to(cuda_device) for t in (codes, scales, zeros)), group=64)
+    want = (x.double() @ fb.w4_weight(codes, scales, zeros, 64).T).to(dtype)
+    for rows in range(1, 36):
+        assert torch.equal(ops.affine_w4(x[:rows].to(cuda_device), w4).cpu(), want[:rows])
+
+
+def test_w4_splits_agree(cuda_device):
+    """Layers that are narrow and deep (a cluster of CTAs per output tile), wide (CTAs that walk over many tiles) and in between."""
+    for n, k in ((16, 16384), (200, 9000), (4096, 640), (20000, 256), (2400, 2304)):
+        for dt, rows in (("bf16", 1), ("f16", 11), ("f32", 2)):
+            x, codes, scales, zeros, b = w4_case(rows, k, n, 128, fb.TYPES[dt], n, True, True)
+            w4 = ops.pack_w4(*(t.to(cuda_device) for t in (codes, scales, zeros)), group=128)
+            want = x.to(cuda_device).double() @ fb.w4_weight(codes, scales, zeros, 128).to(cuda_device).T + b.to(cuda_device).double()
+            assert torch.equal(ops.affine_w4(x.to(cuda_device), w4, b.to(cuda_device)), want.to(fb.TYPES[dt])), (n, k, dt)
+    ops.check_device_flag()
+
+
+def test_another_stream_than_the_current_devices_default(cuda_device):
+    """The work goes to the stream that is current at the call: a long copy in front of it on that stream is waited for."""
+    side = torch.cuda.Stream()
+    src = torch.randn(4096, 4096, device=cuda_device).bfloat16()
+    x = torch.zeros_like(src)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            x.copy_(src)
+            x.zero_()
+        x.copy_(src)
+        ck = ops.checkpoint_code8(x)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(ck.codes, ops.checkpoint_code8(src).codes)

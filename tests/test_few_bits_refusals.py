@@ -33,7 +33,7 @@ def test_checkpoint_refusals():
         st, msg = call("dwbnq_ckpt8_load", *b)
         assert st == status and msg, (i, v, msg)
 
-    for i, vs in {0: (-1, 3, 99), 1: (-1, 1 << 60), 2: (-1, 41, 1 << 60), 3: (39, -1, (1 << 62)), 4: (None, P + 1), 5: (None, P + 8),
+    for i, vs in {0: (-1, 3, 99), 1: (-1, 1 << 60), 2: (-1, 41, 1 << 34), 3: (39, -1, (1 << 62)), 4: (None, P + 1), 5: (None, P + 8),
                   6: (None,)}.items():
         for v in vs:
             bad(i, v)
@@ -68,7 +68,7 @@ def test_affine_backward_refusals():
 
     lib = L.lib()
     for kw in (dict(dtype=7), dict(dw_dtype=L.F16), dict(dtype=L.F32, dw_dtype=L.BF16), dict(rows=-1), dict(rows=1 << 31), dict(c_in=-1),
-               dict(c_out=1 << 25), dict(ld_dy=23)):
+               dict(c_out=1 << 25), dict(ld_dy=23), dict(c_in=1 << 24, c_out=1 << 24, ld_dy=1 << 24)):
         assert run(desc(**kw))[0] == L.ERR_INVALID_ARG, kw
         assert lib.dwbnq_affine_bwd_workspace_bytes(ctypes.byref(desc(**kw))) == 0
     assert call("dwbnq_affine_bwd_ckpt8", None, P, P, P, P, P, 0, P, -1, None)[0] == L.ERR_INVALID_ARG
@@ -87,7 +87,8 @@ def test_w4_refusals():
 
     lib = L.lib()
     for kw, st in ((dict(dtype=3), L.ERR_INVALID_ARG), (dict(group=16), L.ERR_UNSUPPORTED), (dict(group=0), L.ERR_UNSUPPORTED),
-                   (dict(c_in=-1), L.ERR_INVALID_ARG), (dict(c_out=-4), L.ERR_INVALID_ARG), (dict(c_in=1 << 25), L.ERR_INVALID_ARG)):
+                   (dict(c_in=-1), L.ERR_INVALID_ARG), (dict(c_out=-4), L.ERR_INVALID_ARG), (dict(c_in=1 << 25), L.ERR_INVALID_ARG),
+                   (dict(c_in=1 << 23, c_out=1 << 23), L.ERR_INVALID_ARG)):
         d = desc(**kw)
         assert call("dwbnq_w4_pack", ctypes.byref(d), P, P, None, P, -1, None)[0] == st
         assert call("dwbnq_w4_affine_fwd", ctypes.byref(d), 1, 128, P, P, None, 24, P, -1, None)[0] == st
