@@ -246,7 +246,7 @@ __device__ __forceinline__ void store_out(const W4Args &a, int og, int row0, int
 // next, so that memory is kept busy while the warps' sums are added. blockIdx.y: block of 8 NB rows of x. G: group size; ZEROS:
 // zero points. Rows of x that do not exist are read as row 0: their results are columns nobody stores.
 template <typename T, int G, int NB, int R, bool ZEROS>
-__global__ void __launch_bounds__(256) w4_affine_kernel(const W4Args a) {
+__global__ void __launch_bounds__(256, 2) w4_affine_kernel(const W4Args a) {
   using M = W4Math<T>;
   constexpr int GB = kTileI / G;  // quantization groups per block
   constexpr int BLOCK = kTileBytes + GB * kTileO * ((int)sizeof(T) + (ZEROS ? 1 : 0));
@@ -498,22 +498,24 @@ int affine_launch(W4Args a, int warps, int cluster, int ctas, cudaStream_t strea
   const cudaError_t e = cudaLaunchKernelEx(&lc, kern, a);
   return e == cudaSuccess ? DWBNQ_OK : fail_cuda(e, "w4_affine_kernel launch");
 }
-// Output tiles per warp: a warp's rows of x, its waits and its loop cost the same for one tile and for four, so with enough work
-// for every SM (27 blocks) a warp takes as many as its registers allow (4096 -> 14336, one bf16 row: 16.0 us with one, 12.7 with
-// two, 11.4 with four); with less, one, so that more warps share it (512 -> 512: 2.1 us against 3.1). The grid is what then stays
-// resident; where the output tiles are too few for it, a cluster of CTAs divides the input channels of each.
+// Output tiles per warp: a warp's rows of x, its waits and its loop cost the same for one tile and for four, but fewer warps are at
+// work. With enough weights for every SM (27 blocks) a warp takes four tiles where that leaves a group for every SM, else two where
+// that leaves one for every second SM (one bf16 row, us with 4 / 2 tiles: 4096 -> 14336 11.2 / 13.0, 4096 -> 4096 7.6 / 5.1, 14336
+// -> 4096 16.5 / 11.3); with fewer weights one (512 -> 512: 2.1 against 3.1 with four). Rows 9 to 16 double the accumulators: two at
+// most (4096 -> 14336, 16 rows: 19.1 against 25.0). Two CTAs fit an SM; while there are fewer, a cluster of CTAs divides the
+// input channels of each group, and where there are more they walk over the groups in equal rounds.
 template <typename T, int G, bool ZEROS>
 int affine_g(const W4Args &a, cudaStream_t stream) {
-  constexpr int WIDE1 = sizeof(T) == 2 ? 4 : 2, WIDE2 = 2;
   const bool many = (long long)a.o_tiles * a.i_tiles >= 27LL * kPlanSms;
-  const int nb = a.rows > 8 ? 2 : 1, R = !many ? 1 : nb == 2 ? WIDE2 : WIDE1, ogs = (a.o_tiles + R - 1) / R;
-  const int resident = (R == 4 ? 2 : R == 2 ? 3 : 4) * kPlanSms;
+  const int nb = a.rows > 8 ? 2 : 1, R = !many || a.o_tiles < kPlanSms ? 1 : nb == 1 && a.o_tiles >= 4 * kPlanSms ? 4 : 2;
+  const int ogs = (a.o_tiles + R - 1) / R, resident = 2 * kPlanSms;
   int warps = 8, cluster = 1;
   while (warps > 1 && warps > a.i_tiles) warps >>= 1;
   while (cluster < 8 && ogs * cluster * 2 <= resident && a.i_tiles >= 2 * cluster * warps) cluster *= 2;
   const int ctas = resident / cluster;
-  if (nb == 2) return many ? affine_launch<T, G, 2, WIDE2, ZEROS>(a, warps, cluster, ctas, stream) : affine_launch<T, G, 2, 1, ZEROS>(a, warps, cluster, ctas, stream);
-  return many ? affine_launch<T, G, 1, WIDE1, ZEROS>(a, warps, cluster, ctas, stream) : affine_launch<T, G, 1, 1, ZEROS>(a, warps, cluster, ctas, stream);
+  if (nb == 2) return R == 2 ? affine_launch<T, G, 2, 2, ZEROS>(a, warps, cluster, ctas, stream) : affine_launch<T, G, 2, 1, ZEROS>(a, warps, cluster, ctas, stream);
+  return R == 4 ? affine_launch<T, G, 1, 4, ZEROS>(a, warps, cluster, ctas, stream)
+         : R == 2 ? affine_launch<T, G, 1, 2, ZEROS>(a, warps, cluster, ctas, stream) : affine_launch<T, G, 1, 1, ZEROS>(a, warps, cluster, ctas, stream);
 }
 template <typename T, int G>
 int affine_z(const W4Args &a, bool zeros, cudaStream_t stream) {
