@@ -188,7 +188,8 @@ def run(state):
             dw = state["dw"].clone() if case["accum"] else None
             dw, db = ops.affine_weight_backward(ck, state["dy"], dw=dw, need=(True, bool(case["bias"])),
                                                 accum=(bool(case["accum"]), False))
-            return {"dw": dw, "db": db} if case["bias"] else {"dw": dw}
+            # beside a 32-bit dw the call returns db in 32 bits too
+            return {"dw": dw, "db": db.to(t)} if case["bias"] else {"dw": dw}
         return ops.affine_w4(state["x"], state["w4"], state["b"])
 
     if op == "ckpt8":
