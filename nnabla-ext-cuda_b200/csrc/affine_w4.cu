@@ -101,6 +101,10 @@ __global__ void __launch_bounds__(256)
 // one more pair of instructions with an operand of ones, shared by all output channels - is subtracted from the group's sum in
 // fp32. What that costs is the magnitude of the sums, about 30 times the result's: 5 of 24 bits, where the result keeps 8.
 
+// What bounds it: unpacking - 148 instructions per block of 2048 weights, at 16 warps per SM - more than memory. One bf16 row, on
+// the device: 4096 -> 14336 11.1 us (2.7 TB/s), 8192 -> 8192 11.6 us, 4096 -> 4096 5.1 us, 512 -> 512 2.1 us; 16 fp16 rows 8192 ->
+// 8192 with zero points 16.6 us; one float32 row 4096 -> 14336 17.6 us.
+
 template <typename T> struct W4Math {  // bfloat16; float32 in bfloat16 parts
   static constexpr bool OFFSET = sizeof(T) == 2;  // the codes stay 128 above their value
   static constexpr unsigned int MAGIC = 0x43004300u, ONES = 0x3f803f80u;
