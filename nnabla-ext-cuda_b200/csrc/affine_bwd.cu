@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(2 * kTileI)
 }
 
 // ---- bias gradient: CTA (64 channels, slice of the rows), a lane two channels, warp w the rows w, w + 8, ..., eight of them in
-// flight; then the slices in order, a quarter of them per thread and the quarters in order. PAIRS: the two channels of a row are one aligned load ----
+// flight; then the slices in order, a sixteenth of them per thread and those in order. PAIRS: the two channels of a row are one aligned load ----
 constexpr int kDbMaxSlices = 256;
 
 template <typename T, bool PAIRS>
@@ -484,32 +484,36 @@ __global__ void __launch_bounds__(256)
   pdl_launch_dependents();
   pdl_wait_for_predecessor();
   __shared__ float sums[8][64];
-  struct __align__(2 * sizeof(T)) Pair { T a, b; };
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, o = blockIdx.x * 64 + 2 * lane;
   const long long r0 = rows * blockIdx.y / gridDim.y, r1 = rows * (blockIdx.y + 1) / gridDim.y;
   const bool a_ok = o < c_out, b_ok = o + 1 < c_out;
   float s0 = 0.0f, s1 = 0.0f;
-  for (long long t = r0 + w; t < r1; t += 64) {
-    float v[8][2];
+  auto pair = [&](const T *q, float &lo, float &hi) {
+    if constexpr (sizeof(T) == 4) {
+      const float2 e = __ldg(reinterpret_cast<const float2 *>(q));
+      lo = e.x;
+      hi = e.y;
+    } else {
+      unpack_pair(q, __ldg(reinterpret_cast<const unsigned int *>(q)), lo, hi);
+    }
+  };
+  const T *q = dy + (r0 + w) * ld + o;
+  long long t = r0 + w;
+  if (PAIRS && b_ok) {
+    for (; t + 56 < r1; t += 64, q += 64 * ld) {
+      float v[8][2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const T *q = dy + (t + 8 * j) * ld + o;
-      const bool in = t + 8 * j < r1;
-      if (PAIRS && b_ok) {
-        Pair e = {Elem<T>::from_f32(0.0f), Elem<T>::from_f32(0.0f)};
-        if (in) e = *reinterpret_cast<const Pair *>(q);
-        v[j][0] = Elem<T>::to_f32(e.a);
-        v[j][1] = Elem<T>::to_f32(e.b);
-      } else {
-        v[j][0] = in && a_ok ? Elem<T>::to_f32(q[0]) : 0.0f;
-        v[j][1] = in && b_ok ? Elem<T>::to_f32(q[1]) : 0.0f;
+      for (int j = 0; j < 8; ++j) pair(q + 8 * j * ld, v[j][0], v[j][1]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        s0 = __fadd_rn(s0, v[j][0]);
+        s1 = __fadd_rn(s1, v[j][1]);
       }
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      s0 = __fadd_rn(s0, v[j][0]);
-      s1 = __fadd_rn(s1, v[j][1]);
-    }
+  }
+  for (; t < r1; t += 8, q += 8 * ld) {
+    if (a_ok) s0 = __fadd_rn(s0, Elem<T>::to_f32(q[0]));
+    if (b_ok) s1 = __fadd_rn(s1, Elem<T>::to_f32(q[1]));
   }
   sums[w][2 * lane] = s0;
   sums[w][2 * lane + 1] = s1;
@@ -526,20 +530,21 @@ __global__ void __launch_bounds__(256)
     affine_db_join_kernel(const float *__restrict__ part, int slices, int c_out, TW *__restrict__ db, int accum) {
   pdl_launch_dependents();
   pdl_wait_for_predecessor();
-  __shared__ float sums[4][64];
-  const int c = threadIdx.x & 63, q = threadIdx.x >> 6, o = blockIdx.x * 64 + c;
+  __shared__ float sums[16][16];
+  const int c = threadIdx.x & 15, q = threadIdx.x >> 4, o = blockIdx.x * 16 + c;
   float s = 0.0f;
-  for (int i = slices * q / 4, end = slices * (q + 1) / 4; i < end; i += 16) {
-    float v[16];
+  for (int i = slices * q / 16, end = slices * (q + 1) / 16; i < end; i += 8) {
+    float v[8];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = i + j < end && o < c_out ? part[(long long)(i + j) * c_out + o] : 0.0f;
+    for (int j = 0; j < 8; ++j) v[j] = i + j < end && o < c_out ? part[(long long)(i + j) * c_out + o] : 0.0f;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) s = __fadd_rn(s, v[j]);
+    for (int j = 0; j < 8; ++j) s = __fadd_rn(s, v[j]);
   }
   sums[q][c] = s;
   __syncthreads();
   if (q || o >= c_out) return;
-  s = __fadd_rn(__fadd_rn(s, sums[1][c]), __fadd_rn(sums[2][c], sums[3][c]));
+#pragma unroll
+  for (int j = 1; j < 16; ++j) s = __fadd_rn(s, sums[j][c]);
   db[o] = Elem<TW>::from_f32(accum ? __fadd_rn(Elem<TW>::to_f32(db[o]), s) : s);
 }
 
@@ -699,7 +704,7 @@ int run_t(const dwbnq_affine_desc &d, const void *codes, const void *exps, const
     else if (d.dtype == DWBNQ_F16) e = launch_db(d, static_cast<const __half *>(dy), slices, dbp, stream);
     else e = launch_db(d, static_cast<const __nv_bfloat16 *>(dy), slices, dbp, stream);
     if (e != cudaSuccess) return fail_cuda(e, "affine_db_kernel launch");
-    e = launch_pdl(affine_db_join_kernel<TW>, dim3((unsigned)((d.c_out + 63) / 64)), dim3(256), 0, stream, (const float *)dbp, slices, d.c_out,
+    e = launch_pdl(affine_db_join_kernel<TW>, dim3((unsigned)((d.c_out + 15) / 16)), dim3(256), 0, stream, (const float *)dbp, slices, d.c_out,
                    static_cast<TW *>(db), (accum_mask >> 2) & 1);
     if (e != cudaSuccess) return fail_cuda(e, "affine_db_join_kernel launch");
   }
