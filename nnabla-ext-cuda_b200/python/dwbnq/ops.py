@@ -369,8 +369,11 @@ def _rows_view(t, name):
         cols = t.shape[-1]
         if dim == 2:
             rows, (ld, unit) = t.shape[0], t.stride()
-            if rows > 1 and cols > 0 and unit == 1 and ld >= cols:
-                return rows, cols, ld
+            if cols > 0 and unit == 1:
+                if rows == 1:
+                    return 1, cols, cols
+                if rows > 1 and ld >= cols:
+                    return rows, cols, ld
         elif cols > 0:
             return t.numel() // cols, cols, cols
     if dim < 1:
@@ -398,10 +401,11 @@ def _rows_view(t, name):
     return rows, cols, max(ld, cols)
 
 
-def _like(t, name, shape, dtype, device):
-    """A given output (or a second input) checked against what it has to be; a new one when it is None."""
+def _like(t, name, shape, dtype, device, like=None):
+    """A given output (or a second input) checked against what it has to be; a new one when it is None (``like``: a tensor of its
+    type and device, from which it is made faster)."""
     if t is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape) if like is not None else torch.empty(shape, dtype=dtype, device=device)
     if t.shape != shape or t.dtype != dtype:
         raise ValueError("%s must be %s of shape %s, got %s of shape %s" % (name, dtype, tuple(shape), t.dtype, tuple(t.shape)))
     return t
@@ -427,21 +431,22 @@ class Code8Checkpoint:
         self.codes, self.exponents, self.shape, self.dtype, self.rows, self.cols = codes, exponents, shape, dtype, rows, shape[-1]
 
     @classmethod
-    def empty(cls, shape, dtype, device):
+    def empty(cls, shape, dtype, device, like=None):
         ck = cls.__new__(cls)
         rows = 1
         for s in shape[:-1]:
             rows *= s
         groups = (shape[-1] + CODE8_GROUP - 1) // CODE8_GROUP
-        ck.codes = torch.empty((rows, CODE8_GROUP * groups), dtype=torch.int8, device=device)
-        ck.exponents = torch.empty((rows, groups), dtype=torch.uint8, device=device)
+        like = torch.empty(0, device=device) if like is None else like
+        ck.codes = like.new_empty((rows, CODE8_GROUP * groups), dtype=torch.int8)
+        ck.exponents = like.new_empty((rows, groups), dtype=torch.uint8)
         ck.shape, ck.dtype, ck.rows, ck.cols = tuple(shape), dtype, rows, shape[-1]
         return ck
 
 
-def _ck_out(ck, name, shape, dtype, device):
+def _ck_out(ck, name, shape, dtype, like):
     if ck is None:
-        return Code8Checkpoint.empty(shape, dtype, device)
+        return Code8Checkpoint.empty(shape, dtype, like.device, like)
     if ck.shape != tuple(shape) or ck.dtype != dtype:
         raise ValueError("%s must be a checkpoint of a %s tensor of shape %s" % (name, dtype, tuple(shape)))
     return ck
@@ -450,7 +455,7 @@ def _ck_out(ck, name, shape, dtype, device):
 def checkpoint_code8(x, out=None):
     """The 8-bit checkpoint of x [..., channels] (groups of 32 channels share a power-of-two step)."""
     code = _few_bits_code(x.dtype)
-    ck = _ck_out(out, "out", x.shape, x.dtype, x.device)
+    ck = _ck_out(out, "out", x.shape, x.dtype, x)
     dev = _one_device(x, ck.codes, ck.exponents)
     rows, cols, ld = _rows_view(x, "x")
     _launch("dwbnq_ckpt8_store", dev, code, rows, cols, ld, x.data_ptr(), ck.codes.data_ptr(), ck.exponents.data_ptr())
@@ -472,14 +477,14 @@ def glu(gate, up, act="silu", checkpoint=False, out=None):
     checkpoint of gate, checkpoint of up), all written in one pass. ``out`` may be ``gate`` or ``up``."""
     code = _few_bits_code(gate.dtype)
     _like(up, "up", gate.shape, gate.dtype, gate.device)
-    y = _like(out, "out", gate.shape, gate.dtype, gate.device)
+    y = _like(out, "out", gate.shape, gate.dtype, gate.device, gate)
     dev = _one_device(gate, up, y)
     (rows, cols, ldg), (_, _, ldu), (_, _, ldy) = _rows_view(gate, "gate"), _rows_view(up, "up"), _rows_view(y, "out")
     if not checkpoint:
         _launch("dwbnq_glu_fwd", dev, code, _GLU_ACTS[act], rows, cols, ldg, gate.data_ptr(), ldu, up.data_ptr(), ldy,
                 y.data_ptr(), None, None, None, None)
         return y
-    cg, cu = (Code8Checkpoint.empty(gate.shape, gate.dtype, dev) for _ in range(2))
+    cg, cu = (Code8Checkpoint.empty(gate.shape, gate.dtype, dev, gate) for _ in range(2))
     _launch("dwbnq_glu_fwd", dev, code, _GLU_ACTS[act], rows, cols, ldg, gate.data_ptr(), ldu, up.data_ptr(), ldy, y.data_ptr(),
             cg.codes.data_ptr(), cg.exponents.data_ptr(), cu.codes.data_ptr(), cu.exponents.data_ptr())
     return y, cg, cu
@@ -503,14 +508,14 @@ def glu_backward(ck_gate, ck_up, dy, act="silu", product=False, dgate=None, dup=
     ldd = ldg = ldu = cols
     if dy is not None:
         ldd = _rows_view(_like(dy, "dy", shape, dtype, device), "dy")[2]
-    dgate = _like(dgate, "dgate", shape, dtype, device) if need[0] else None
-    dup = _like(dup, "dup", shape, dtype, device) if need[1] else None
+    dgate = _like(dgate, "dgate", shape, dtype, device, dy) if need[0] else None
+    dup = _like(dup, "dup", shape, dtype, device, dy) if need[1] else None
     if dgate is not None:
         ldg = _rows_view(dgate, "dgate")[2]
     if dup is not None:
         ldu = _rows_view(dup, "dup")[2]
     dev = _one_device(ck_gate.codes, ck_gate.exponents, ck_up.codes, ck_up.exponents, dy, dgate, dup)
-    ck = Code8Checkpoint.empty(shape, dtype, dev) if product else None
+    ck = Code8Checkpoint.empty(shape, dtype, dev, ck_gate.codes) if product else None
     mask = (1 if accum[0] else 0) | (2 if accum[1] else 0)
     _launch("dwbnq_glu_bwd_ckpt8", dev, code, _GLU_ACTS[act], ck_gate.rows, cols, ck_gate.codes.data_ptr(),
             ck_gate.exponents.data_ptr(), ck_up.codes.data_ptr(), ck_up.exponents.data_ptr(), ldd, _addr(dy), ldg, _addr(dgate),
@@ -536,8 +541,9 @@ def affine_weight_backward(ck_x, dy, dw=None, db=None, need=(True, True), accum=
         dtype = dw.dtype if dw is not None else db.dtype if db is not None else dy.dtype
     rows, c_out, ld = _rows_view(dy, "dy")
     c_in = ck_x.cols
-    dw = _like(dw, "dw", (c_out, c_in), dtype, dy.device) if need[0] else None
-    db = _like(db, "db", (c_out,), dtype, dy.device) if need[1] else None
+    like = dy if dtype == dy.dtype else None
+    dw = _like(dw, "dw", (c_out, c_in), dtype, dy.device, like) if need[0] else None
+    db = _like(db, "db", (c_out,), dtype, dy.device, like) if need[1] else None
     for t, n in ((dw, "dw"), (db, "db")):
         if t is not None and not t.is_contiguous():
             raise ValueError("%s must be contiguous" % n)
@@ -607,7 +613,7 @@ def affine_w4(x, w4, b=None, out=None):
     rows, c_in, ldx = _rows_view(x, "x")
     if c_in != w4.c_in:
         raise ValueError("x has %d channels, the weights %d" % (c_in, w4.c_in))
-    y = _like(out, "out", tuple(x.shape[:-1]) + (w4.c_out,), x.dtype, x.device)
+    y = _like(out, "out", x.shape[:-1] + (w4.c_out,), x.dtype, x.device, x)
     if b is not None and not _like(b, "b", (w4.c_out,), x.dtype, x.device).is_contiguous():
         raise ValueError("b must be contiguous")
     dev = _one_device(x, w4.packed, b, y)
