@@ -18,7 +18,7 @@
 //    are added to dw in fp32: the tensor core's adder truncates, by 2^-25 of the sum per step of 16 tokens on
 //    average, and over a long batch that would be the result's error;
 //  * what bounds it: the way of a stage - copy 1600 cycles, expansion 800, issue and MMAs 1000 - against the four stages that fit;
-//    8192 tokens, 4096 x 4096, bf16: 256 us, 1072 TFLOP/s (317 us with a 32-bit result; fp16 920 us, fp32 1250 us: there the split of
+//    8192 tokens, 4096 x 4096, bf16: 256 us, 1072 TFLOP/s (317 us with a 32-bit result; fp16 855 us, fp32 1290 us: there the split of
 //    dy into parts is most of the work);
 //  * tiles that fill whole waves of the 148 SMs are walked as they are; the tiles of the last, partial wave
 //    are cut along the tokens so that it is full too, and a second kernel adds their parts in a fixed order.
@@ -184,11 +184,12 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
   static_assert(DY == DY_TMA || BN == 128, "a lane splits eight columns of a row");
   static_assert(STAGE % 1024 == 0 && STAGES * STAGE + 2048 <= kSmemMax, "swizzle atoms; shared memory");
   extern __shared__ unsigned char smem_raw[];
-  __shared__ unsigned long long bars[3 * kMaxStages + 2 * kMaxAcc + 1];
+  __shared__ unsigned long long bars[4 * kMaxStages + 2 * kMaxAcc + 1];
   __shared__ unsigned int tmem_base_s;
   __shared__ int abort_s;
   unsigned long long *full = bars, *empty = bars + kMaxStages, *conv = bars + 2 * kMaxStages;
-  unsigned long long *acc_full = bars + 3 * kMaxStages, *acc_empty = acc_full + kMaxAcc, *drained = acc_empty + kMaxAcc;
+  unsigned long long *raw_empty = bars + 3 * kMaxStages;  // DY_RAW: what TMA brought has been read
+  unsigned long long *acc_full = bars + 4 * kMaxStages, *acc_empty = acc_full + kMaxAcc, *drained = acc_empty + kMaxAcc;
   const unsigned int base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char *sm = smem_raw + (base - smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -198,6 +199,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
       mbar_init(&conv[s], GROUP);
+      mbar_init(&raw_empty[s], GROUP);
     }
     for (int b = 0; b < NACC; ++b) {
       mbar_init(&acc_full[b], 1);
@@ -233,7 +235,8 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
       constexpr int COLS = DyBox<T>::COLS, MAXBOX = BN / COLS, DYAT = DY == DY_RAW ? S::RAW : XB;
       const int boxes = DY == DY_LOAD ? 0 : min(MAXBOX, (a.c_out - o0 + COLS - 1) / COLS);
       for (int c = c0; c < c1; ++c) {
-        if (!dw_wait(&empty[s], ph ^ 1u, abort_v)) { ok = false; break; }
+        // where dy is split, its raw form and the codes may be replaced once they are split, not only when the MMAs are through
+        if (!dw_wait(DY == DY_RAW ? &raw_empty[s] : &empty[s], ph ^ 1u, abort_v)) { ok = false; break; }
         if (elect_one()) {
           unsigned char *st = sm + s * STAGE;
           mbar_expect_tx(&full[s], (boxes + 1) * BOX);
@@ -347,7 +350,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
       const int c_now = c, o = tile / a.i_tiles * BN + l16 * 8;
       move(STAGES);
       exponents(ex_next);
-      if (!dw_wait(&full[g], ph, abort_v)) { ok = false; break; }
+      if (!dw_wait(&full[g], ph, abort_v) || (DY == DY_RAW && !dw_wait(&empty[g], ph ^ 1u, abort_v))) { ok = false; break; }
 #pragma unroll
       for (int p = 0; p < TOKENS / 2; ++p) {
         const unsigned int r = tok0 + 2 * p + hi;
@@ -374,6 +377,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // visible to the tensor core's reads
       __syncwarp();
+      if (DY == DY_RAW && lane == 0) mbar_arrive(&raw_empty[g]);
       if (lane == 0) mbar_arrive(&conv[g]);
 #pragma unroll
       for (int k = 0; k < EX; ++k) ex[k] = ex_next[k];

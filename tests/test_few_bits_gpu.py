@@ -598,3 +598,63 @@ def test_another_stream_than_the_current_devices_default(cuda_device):
         ck = ops.checkpoint_code8(x)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(ck.codes, ops.checkpoint_code8(src).codes)
+
+
+class Fenced:
+    """Tensors between two bands of a known pattern."""
+
+    BAND = 4096
+
+    def __init__(self, device):
+        self.device, self.buffers = device, []
+
+    def __call__(self, shape, dtype, fill=None):
+        n = int(np.prod(shape)) * torch.empty(0, dtype=dtype).element_size()
+        buf = torch.full((self.BAND + (n + 255) // 256 * 256 + self.BAND,), 0xA5, dtype=torch.uint8, device=self.device)
+        self.buffers.append((buf, n))
+        t = buf[self.BAND:self.BAND + n].view(dtype).view(shape)
+        if fill is not None:
+            t.copy_(fill)
+        return t
+
+    def check(self):
+        for buf, n in self.buffers:
+            assert (buf[:self.BAND] == 0xA5).all() and (buf[self.BAND + n:] == 0xA5).all()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows,c_in,c_out", [(1, 1, 1), (65, 100, 36), (130, 257, 300), (1027, 64, 513)])
+def test_nothing_beside_the_tensors_is_written(cuda_device, dt, rows, c_in, c_out):
+    import ctypes
+
+    from dwbnq import _lib as L
+    dtype, fence = fb.TYPES[dt], Fenced(cuda_device)
+    groups = (c_in + 31) // 32
+    x = fence((rows, c_in), dtype, activations(rows, c_in, dtype, 1))
+    up = fence((rows, c_in), dtype, activations(rows, c_in, dtype, 2))
+    dy = fence((rows, c_out), dtype, activations(rows, c_out, dtype, 3))
+    ck = [ops.Code8Checkpoint(fence((rows, 32 * groups), torch.int8), fence((rows, groups), torch.uint8), (rows, c_in), dtype) for _ in range(3)]
+    y, dg, du = (fence((rows, c_in), dtype) for _ in range(3))
+    ops.checkpoint_code8(x, out=ck[0])
+    ops.restore_code8(ck[0], out=y)
+    lib, stream = L.lib(), torch.cuda.current_stream().cuda_stream
+    ptr = lambda c: (c.codes.data_ptr(), c.exponents.data_ptr())  # noqa: E731
+    code = L.BF16 if dt == "bf16" else L.F16 if dt == "f16" else L.F32
+    L.check(lib.dwbnq_glu_fwd(code, L.ACT_GELU, rows, c_in, c_in, x.data_ptr(), c_in, up.data_ptr(), c_in, y.data_ptr(), *ptr(ck[0]), *ptr(ck[1]),
+                              0, stream))
+    L.check(lib.dwbnq_glu_bwd_ckpt8(code, L.ACT_GELU, rows, c_in, *ptr(ck[0]), *ptr(ck[1]), c_in, y.data_ptr(), c_in, dg.data_ptr(), c_in,
+                                    du.data_ptr(), *ptr(ck[2]), 3 if rows % 2 else 0, 0, stream))
+    for out in {code, L.F32}:
+        d = L.AffineDesc(dtype=code, dw_dtype=out, rows=rows, c_in=c_in, c_out=c_out, ld_dy=c_out)
+        t = torch.float32 if out == L.F32 else dtype
+        ws = fence((int(lib.dwbnq_affine_bwd_workspace_bytes(ctypes.byref(d))),), torch.uint8)
+        ops.affine_weight_backward(ck[0], dy, dw=fence((c_out, c_in), t), db=fence((c_out,), t), ws=ws)
+    q, s = ops.quantize_w4(x, group=64)
+    w4 = ops.pack_w4(q, s, group=64)
+    w4.packed = fence(tuple(w4.packed.shape), torch.uint8, w4.packed)
+    for r in (1, 9, 20):
+        xs = fence((r, c_in), dtype, activations(r, c_in, dtype, 4))
+        ops.affine_w4(xs, w4, out=fence((r, rows), dtype))
+    torch.cuda.synchronize()
+    fence.check()
+    ops.check_device_flag()
