@@ -4,22 +4,22 @@
 // The weight gradient is a product contracted over the tokens, D[i][o] = X^T dY, on the 5th-generation
 // tensor cores (tcgen05.mma.kind::f16, both factors bfloat16, fp32 accumulators in tensor memory):
 //  * the value of a checkpoint is exact in bfloat16, and so is every product; dy is taken as it is
-//    (bfloat16), or as the exact sum of two (float16) or three (float32) bfloat16 parts, one pass each;
+//    (bfloat16), or as the exact sum of two (float16) or three (float32) bfloat16 parts, written once by a kernel of
+//    its own and contracted one after the other, the smallest first;
 //  * the 128 accumulator rows are input channels and the columns output channels: a warp that reads the
 //    accumulator back holds 32 consecutive elements of one row of dw per column, so every store is a
 //    coalesced line and nothing is staged. Both factors are MN-major in shared memory, as they lie in
 //    global memory: no transpose anywhere;
 //  * per CTA (one per SM): warp 0 issues the TMA loads, warp 1 the MMAs, warps 2-17 expand the codes into the
-//    swizzled operand layout (and split dy where it is not bfloat16 or its rows are not multiples of 16 bytes),
-//    warps 18-25 read the accumulators back. The converters work in as many groups as there are stages, a
-//    chunk of 64 tokens per group: one warp needs about 1400 cycles from its wait to its next one, and with all
-//    of them on every chunk that was the kernel's pace (512 cycles of MMAs per chunk);
+//    swizzled operand layout, warps 18-25 read the accumulators back. The converters work in as many groups as
+//    there are stages, a chunk of 64 tokens per group: one warp needs about 1400 cycles from its wait to its next
+//    one, and with all of them on every chunk that was the kernel's pace (512 cycles of MMAs per chunk);
 //  * where the result is kept in 32 bits, the accumulator is read back after a run of a few chunks and the runs
 //    are added to dw in fp32: the tensor core's adder truncates, by 2^-25 of the sum per step of 16 tokens on
 //    average, and over a long batch that would be the result's error;
 //  * what bounds it: the way of a stage - copy 1600 cycles, expansion 800, issue and MMAs 1000 - against the four stages that fit;
-//    8192 tokens, 4096 x 4096, bf16: 256 us, 1072 TFLOP/s (317 us with a 32-bit result; fp16 855 us, fp32 1290 us: there the split of
-//    dy into parts is most of the work);
+//    8192 tokens, 4096 x 4096, bf16: 256 us, 1072 TFLOP/s (322 us with a 32-bit result; fp16 509 us, two products; fp32 1026 us,
+//    three products, and 4 GB of partial results through L2);
 //  * tiles that fill whole waves of the 148 SMs are walked as they are; the tiles of the last, partial wave
 //    are cut along the tokens so that it is full too, and a second kernel adds their parts in a fixed order.
 #include <cstring>
@@ -33,20 +33,26 @@ namespace dwbnq {
 namespace {
 
 constexpr int kTileI = 128;       // input channels per tile = TMEM lanes
+constexpr int kChunk = 64;        // tokens per pipeline stage
+// Chunks per run of a result kept in 32 bits. What the adder drops is relative to the sum, so the parts of dy below the leading
+// digits (at most 2^-7 of it) may run longer; a float32 dy is held to half of what 16 bits are.
+constexpr int kRun = 16, kRunF32 = 8, kLowRun = 64;
 constexpr int kConvWarps = 16, kFirstEpi = 2 + kConvWarps, kEpiWarps = 8;
 constexpr int kThreads = 32 * (kFirstEpi + kEpiWarps);
-constexpr int kMaxStages = 4, kTmemCols = 512, kMaxAcc = 4;
+constexpr int kTmemCols = 512;
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kPlanSms = 148;     // SMs of a B200: the cut of the last wave does not depend on the device it is asked on
 constexpr int kMaxParts = 2 * kPlanSms;
 
 struct DwArgs {
   const unsigned char *exps;
-  const void *dy;
-  long long ld, rows;
+  long long rows;
   int c_in, c_out, groups;
   int i_tiles;
-  int chunks;              // ceil(rows / tokens per chunk)
+  int token_chunks;        // ceil(rows / 64)
+  int chunks;              // of a tile: token_chunks of every bfloat16 part of dy, the smallest part first
+  int head;                // the first chunk of the part that holds dy's leading digits
+  int run;                 // chunks per run there
   int full, segs, units;   // units 0 .. full-1: whole tiles; then segs parts of every further tile
   void *dw;
   float *parts;            // [unit - full][tile columns][128]
@@ -121,46 +127,34 @@ __device__ __forceinline__ void dw_split(float *v, uint4 *part) {
   }
 }
 
-// How dy reaches the tensor cores: by TMA as it is (bfloat16); by TMA into a buffer from which the converters split it (float16,
-// float32); or loaded and split by the converters (rows that are not multiples of 16 bytes, which TMA cannot take).
-enum DyMode : int { DY_TMA = 0, DY_RAW = 1, DY_LOAD = 2 };
-template <typename T> struct DyBox { static constexpr int COLS = 128 / (int)sizeof(T); };  // a box is a chunk's tokens x 128 bytes
-// Tokens per pipeline stage: where dy is split a stage also holds it as it came and in parts, and four stages of 32 tokens
-// cover the loads' latency better than two of 64.
-__host__ __device__ constexpr int dw_chunk(int dy_mode) { return dy_mode == DY_TMA ? 64 : 32; }
+// dy as bfloat16 parts [PARTS][rows][pad] (pad: c_out up to a multiple of 8), which TMA can take whatever dy's type, address and row
+// stride. A pass of its own: splitting inside the product kernel was done again for every tile of input channels, and with the
+// parts beside dy itself in shared memory the pipeline was half as deep (8192 tokens, 4096 x 4096 fp16: 855 us against 509).
+template <typename T, int PARTS, bool VECTORS>
+__global__ void __launch_bounds__(256)
+    affine_split_kernel(const T *__restrict__ dy, long long ld, long long rows, int c_out, const OctetGrid g, long long pad,
+                        uint4 *__restrict__ out) {
+  pdl_launch_dependents();
+  pdl_wait_for_predecessor();
+  float *stage = OctetStage<VECTORS>::get();
+  for (OctetWalk w = octet_walk(g, rows); __any_sync(0xffffffffu, w.row < rows); octet_next(w)) {
+    const bool in = w.row < rows;
+    const long long c = w.col * 8LL;
+    float v[8];
+    Octet<T, VECTORS>::load(dy + w.row * ld + c, in ? c_out - c : 0, stage, v);
+    uint4 part[PARTS];
+    dw_split<PARTS>(v, part);
+    if (in && c < pad)
+#pragma unroll
+      for (int q = 0; q < PARTS; ++q) out[((q * rows + w.row) * pad + c) / 8] = part[q];
+  }
+}
 
-// Eight consecutive elements of a row of dy.
-template <typename T> struct DyVec {
-  uint4 w[8 * (int)sizeof(T) / 16];
-  // elements 8 i .. 8 i + 7 of row r of the boxes at `raw`; zero beyond the tensor, as TMA filled them
-  __device__ __forceinline__ void load_shared(const unsigned char *raw, unsigned int r, int i) {
-    constexpr int PER = DyBox<T>::COLS / 8;  // vectors per box row
-    const uint4 *p = reinterpret_cast<const uint4 *>(raw + (i / PER) * (dw_chunk(DY_RAW) * 128) + r * 128 + (i % PER) * 8 * sizeof(T));
-#pragma unroll
-    for (int k = 0; k < 8 * (int)sizeof(T) / 16; ++k) w[k] = p[k];
-  }
-  // columns col .. col + 7 of a row of global memory; zero from column n on
-  __device__ __forceinline__ void load(const T *row, int col, int n) {
-    T e[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = col + j < n ? __ldg(row + col + j) : Elem<T>::from_f32(0.0f);
-    memcpy(w, e, sizeof(w));
-  }
-  __device__ __forceinline__ void get(float *v) const {
-    T e[8];
-    memcpy(e, w, sizeof(w));
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = Elem<T>::to_f32(e[j]);
-  }
-};
-
-// A stage holds the expanded codes, the parts of dy, the codes, and dy as it came where it is split. Two or four stages: the
-// converters' groups are as many, so that each stage's barriers are always awaited by the same group (a parity wait cannot
-// tell a phase from the one after the next).
-template <int PARTS, int BN, int DY, int TBYTES> struct DwStage {
-  static constexpr int CHUNK = dw_chunk(DY), XB = CHUNK * kTileI * 2, DYB = CHUNK * BN * 2, CODES = XB + PARTS * DYB,
-                       RAW = CODES + CHUNK * kTileI, BYTES = RAW + (DY == DY_RAW ? CHUNK * BN * TBYTES : 0), COUNT = 4 * BYTES + 2048 <= kSmemMax ? 4 : 2;
-};
+// A stage holds the expanded codes, dy, and the codes. Four stages and as many groups of converters, so that each stage's barriers are
+// always awaited by the same group (a parity wait cannot tell a phase from the one after the next).
+constexpr int kBn = 256, kXBytes = kChunk * kTileI * 2, kDyBytes = kChunk * kBn * 2, kStageBytes = kXBytes + kDyBytes + kChunk * kTileI;
+constexpr int kStages = 4, kBox = kChunk * 128;  // a box: 64 tokens x 128 bytes
+static_assert(kStageBytes % 1024 == 0 && kStages * kStageBytes + 2048 <= kSmemMax, "swizzle atoms; shared memory");
 
 // pw_wait for a warp of a CTA that may be giving up: the flag is looked at only when the barrier is not ready.
 __device__ __forceinline__ bool dw_wait(unsigned long long *bar, unsigned int parity, volatile int *abort_v) {
@@ -168,38 +162,29 @@ __device__ __forceinline__ bool dw_wait(unsigned long long *bar, unsigned int pa
   return pw_wait(bar, parity) && !*abort_v;
 }
 
-// T: type of dy; TW: type of dw (32 bits: sums in short runs); PARTS: bfloat16 parts of dy; BN: output channels per tile.
-template <typename T, typename TW, int PARTS, int DY, int BN>
+// TW: type of dw (32 bits: sums in short runs).
+template <typename TW>
 __global__ void __launch_bounds__(kThreads, 1)
 affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ CUtensorMap tm_codes, const DwArgs a) {
-  using S = DwStage<PARTS, BN, DY, (int)sizeof(T)>;
-  constexpr int CHUNK = S::CHUNK, XB = S::XB, DYB = S::DYB, STAGE = S::BYTES, STAGES = S::COUNT;
-  constexpr int BOX = CHUNK * 128;                    // bytes of a box of CHUNK tokens
-  constexpr int GROUP = kConvWarps / STAGES, TOKENS = CHUNK / GROUP;  // converter warps per group, tokens per warp and chunk
+  constexpr int BN = kBn, GROUP = kConvWarps / kStages, TOKENS = kChunk / GROUP;  // converter warps per group, tokens per warp and chunk
   constexpr bool KEEP32 = sizeof(TW) == 4;
-  constexpr int RUN = (PARTS == 1 ? 1024 : PARTS == 2 ? 512 : 256) / CHUNK;  // chunks per run: the more digits in dy, the more the adder drops
-  constexpr int NACC = kTmemCols / BN < kMaxAcc ? kTmemCols / BN : kMaxAcc;
+  constexpr int NACC = kTmemCols / BN;
   constexpr int HALF = BN / 2;                        // columns per epilogue warp
-  static_assert(DY != DY_TMA || PARTS == 1, "dy as it is has one part");
-  static_assert(DY == DY_TMA || BN == 128, "a lane splits eight columns of a row");
-  static_assert(STAGE % 1024 == 0 && STAGES * STAGE + 2048 <= kSmemMax, "swizzle atoms; shared memory");
   extern __shared__ unsigned char smem_raw[];
-  __shared__ unsigned long long bars[4 * kMaxStages + 2 * kMaxAcc + 1];
+  __shared__ unsigned long long bars[3 * kStages + 2 * NACC + 1];
   __shared__ unsigned int tmem_base_s;
   __shared__ int abort_s;
-  unsigned long long *full = bars, *empty = bars + kMaxStages, *conv = bars + 2 * kMaxStages;
-  unsigned long long *raw_empty = bars + 3 * kMaxStages;  // DY_RAW: what TMA brought has been read
-  unsigned long long *acc_full = bars + 4 * kMaxStages, *acc_empty = acc_full + kMaxAcc, *drained = acc_empty + kMaxAcc;
+  unsigned long long *full = bars, *empty = bars + kStages, *conv = bars + 2 * kStages;
+  unsigned long long *acc_full = bars + 3 * kStages, *acc_empty = acc_full + NACC, *drained = acc_empty + NACC;
   const unsigned int base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char *sm = smem_raw + (base - smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
       mbar_init(&conv[s], GROUP);
-      mbar_init(&raw_empty[s], GROUP);
     }
     for (int b = 0; b < NACC; ++b) {
       mbar_init(&acc_full[b], 1);
@@ -224,7 +209,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
   volatile int *abort_v = &abort_s;
 
   if (warp == 0) {
-    // ---- TMA loads: the codes and, where it can take them, dy: boxes of a chunk's tokens x 128 bytes, zero beyond the tensors ----
+    // ---- TMA loads, boxes of 64 tokens x 128 bytes, zero beyond the tensors: the codes, and dy or one of its parts ----
     int s = 0, issued = 0;
     unsigned int ph = 0;
     bool ok = true;
@@ -232,29 +217,29 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
       int tile, c0, c1;
       dw_unit(a, u, tile, c0, c1);
       const int ot = tile / a.i_tiles, o0 = ot * BN, i0 = (tile - ot * a.i_tiles) * kTileI;
-      constexpr int COLS = DyBox<T>::COLS, MAXBOX = BN / COLS, DYAT = DY == DY_RAW ? S::RAW : XB;
-      const int boxes = DY == DY_LOAD ? 0 : min(MAXBOX, (a.c_out - o0 + COLS - 1) / COLS);
+      const int boxes = min(BN / 64, (a.c_out - o0 + 63) / 64);
+      int part = a.chunks / a.token_chunks - 1 - c0 / a.token_chunks, ct = c0 % a.token_chunks;
       for (int c = c0; c < c1; ++c) {
-        // where dy is split, its raw form and the codes may be replaced once they are split, not only when the MMAs are through
-        if (!dw_wait(DY == DY_RAW ? &raw_empty[s] : &empty[s], ph ^ 1u, abort_v)) { ok = false; break; }
+        if (!dw_wait(&empty[s], ph ^ 1u, abort_v)) { ok = false; break; }
         if (elect_one()) {
-          unsigned char *st = sm + s * STAGE;
-          mbar_expect_tx(&full[s], (boxes + 1) * BOX);
-          tma_load_2d(st + S::CODES, &tm_codes, i0, c * CHUNK, &full[s]);
+          unsigned char *st = sm + s * kStageBytes;
+          mbar_expect_tx(&full[s], (boxes + 1) * kBox);
+          tma_load_2d(st + kXBytes + kDyBytes, &tm_codes, i0, ct * kChunk, &full[s]);
 #pragma unroll
-          for (int q = 0; q < MAXBOX; ++q)
-            if (q < boxes) tma_load_2d(st + DYAT + q * BOX, &tm_dy, o0 + q * COLS, c * CHUNK, &full[s]);
+          for (int q = 0; q < BN / 64; ++q)
+            if (q < boxes) tma_load_3d(st + kXBytes + q * kBox, &tm_dy, o0 + q * 64, ct * kChunk, part, &full[s]);
         }
         __syncwarp();
-        if (issued < STAGES) ++issued;
-        if (++s == STAGES) { s = 0; ph ^= 1u; }
+        if (++ct == a.token_chunks) { ct = 0; --part; }
+        if (issued < kStages) ++issued;
+        if (++s == kStages) { s = 0; ph ^= 1u; }
       }
     }
     if (!ok && lane == 0) {
       if (!*abort_v) { atomicExch(a.flag, 1); *abort_v = 1; }
       // the copies in flight land before the CTA gives its shared memory back
       for (; issued > 0; --issued) {
-        if (--s < 0) { s = STAGES - 1; ph ^= 1u; }
+        if (--s < 0) { s = kStages - 1; ph ^= 1u; }
         pw_wait_lane(&full[s], ph);
       }
     }
@@ -262,7 +247,8 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
     // ---- MMAs: the warp walks through the chunks, one elected lane issues ----
     // fp32 accumulator, bfloat16 factors, both MN-major, M = 128; N is set per tile
     const unsigned int idesc0 = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | (8u << 24);
-    const unsigned long long dx0 = pw_smem_desc(base, BOX, 1024, 2), dd0 = pw_smem_desc(base + XB, BOX, 1024, 2);
+    const unsigned long long dx0 = pw_smem_desc(base, kBox, 1024, 2), dd0 = pw_smem_desc(base + kXBytes, kBox, 1024, 2);
+    const int last_steps = (int)((a.rows - (long long)(a.token_chunks - 1) * kChunk + 15) / 16);
     int s = 0, b = 0;
     unsigned int ph = 0, aph = 0;
     bool ok = true;
@@ -272,24 +258,20 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
       const int o0 = tile / a.i_tiles * BN;
       const int n = min(BN, (a.c_out - o0 + 15) & ~15);
       const unsigned int idesc = idesc0 | ((unsigned)(n >> 3) << 17);
-      int run = 0;
+      int run = 0, ct = c0 % a.token_chunks;
       for (int c = c0; c < c1; ++c) {
         // dy and the codes of the stage have landed when its converters have arrived: they waited for them
         if ((run == 0 && !dw_wait(&acc_empty[b], aph ^ 1u, abort_v)) || !dw_wait(&conv[s], ph, abort_v)) { ok = false; break; }
         tc_fence_after();
-        const bool last = c == c1 - 1 || (KEEP32 && run == RUN - 1);
-        const unsigned long long so = (unsigned long long)(s * STAGE) >> 4;
+        const bool last = c == c1 - 1 || (KEEP32 && (run == (c < a.head ? kLowRun : a.run) - 1 || c == a.head - 1));
+        const int steps = ++ct == a.token_chunks ? last_steps : kChunk / 16;
+        const unsigned long long so = (unsigned long long)(s * kStageBytes) >> 4, dx = dx0 + so, dd = dd0 + so;
         const unsigned int d = tmem_base + b * BN;
-        const int steps = (int)min((long long)CHUNK / 16, (a.rows - (long long)c * CHUNK + 15) / 16);
+        if (ct == a.token_chunks) ct = 0;
         if (elect_one()) {
-          // the small parts first: a sum that only grows loses least
 #pragma unroll
-          for (int p = PARTS - 1; p >= 0; --p) {
-            const unsigned long long dx = dx0 + so, dd = dd0 + so + (unsigned)(p * (DYB >> 4));
-#pragma unroll
-            for (int j = 0; j < CHUNK / 16; ++j)  // a step is 16 rows of 128 bytes
-              if (j == 0 || j < steps) tc_mma_f16(d, dx + j * 128, dd + j * 128, idesc, j || p < PARTS - 1 ? 1u : run ? 1u : 0u);
-          }
+          for (int j = 0; j < kChunk / 16; ++j)  // a step is 16 rows of 128 bytes
+            if (j == 0 || j < steps) tc_mma_f16(d, dx + j * 128, dd + j * 128, idesc, j ? 1u : run ? 1u : 0u);
           tc_commit(&empty[s]);
           if (last) tc_commit(&acc_full[b]);
         }
@@ -299,7 +281,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
           run = 0;
           if (++b == NACC) { b = 0; aph ^= 1u; }
         }
-        if (++s == STAGES) { s = 0; ph ^= 1u; }
+        if (++s == kStages) { s = 0; ph ^= 1u; }
       }
     }
     if (!ok) {
@@ -309,13 +291,13 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
       pw_wait(drained, 0);
     }
   } else if (warp < kFirstEpi) {
-    // ---- converters: group g has the chunks n = g, g + STAGES, ... of this CTA and with them stage g; a warp has TOKENS tokens
+    // ---- converters: group g has the chunks n = g, g + kStages, ... of this CTA and with them stage g; a warp has TOKENS tokens
     // of the chunk, a pass is two tokens, a lane eight channels. The exponents of a warp's tokens come by byte loads, one chunk
     // of the group ahead. The code is kept short: unrolled over several chunks it threw the instructions of the warps that
     // issue the loads and the MMAs out of the instruction cache ----
     const int g = (warp - 2) / GROUP, l16 = lane & 15, hi = lane >> 4;
-    const unsigned int tok0 = ((warp - 2) % GROUP) * TOKENS, box = (l16 >> 3) * (unsigned)BOX;
-    unsigned char *st = sm + g * STAGE;
+    const unsigned int tok0 = ((warp - 2) % GROUP) * TOKENS, box = (l16 >> 3) * (unsigned)kBox;
+    unsigned char *st = sm + g * kStageBytes;
     static_assert(TOKENS >= 8, "a byte of exponents for every lane");
     constexpr int EX = TOKENS * 4 / 32;  // exponents per lane: four groups of 32 channels per token
     int u = blockIdx.x, tile = 0, c = 0, c1 = 0;
@@ -336,7 +318,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
       const int gr = tile % a.i_tiles * (kTileI / kCkGroup) + (lane & 3);
 #pragma unroll
       for (int k = 0; k < EX; ++k) {
-        const long long t = (long long)c * CHUNK + tok0 + k * 8 + (lane >> 2);
+        const long long t = (long long)(c % a.token_chunks) * kChunk + tok0 + k * 8 + (lane >> 2);
         e[k] = u < a.units && t < a.rows && gr < a.groups ? __ldg(a.exps + t * a.groups + gr) : kCkMinExp;
       }
     };
@@ -347,37 +329,18 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
     exponents(ex);
     bool ok = true;
     while (u < a.units) {
-      const int c_now = c, o = tile / a.i_tiles * BN + l16 * 8;
-      move(STAGES);
+      move(kStages);
       exponents(ex_next);
-      if (!dw_wait(&full[g], ph, abort_v) || (DY == DY_RAW && !dw_wait(&empty[g], ph ^ 1u, abort_v))) { ok = false; break; }
+      if (!dw_wait(&full[g], ph, abort_v)) { ok = false; break; }
 #pragma unroll
       for (int p = 0; p < TOKENS / 2; ++p) {
         const unsigned int r = tok0 + 2 * p + hi;
-        const uint2 code = *reinterpret_cast<const uint2 *>(st + S::CODES + r * kTileI + l16 * 8);
+        const uint2 code = *reinterpret_cast<const uint2 *>(st + kXBytes + kDyBytes + r * kTileI + l16 * 8);
         const unsigned int e = __shfl_sync(0xffffffffu, ex[p / 4], (2 * (p & 3) + hi) * 4 + (l16 >> 2));
         *reinterpret_cast<uint4 *>(st + box + r * 128 + (((l16 & 7) ^ (r & 7)) << 4)) = dw_expand(code, e, magic);
       }
-      if (DY != DY_TMA) {
-#pragma unroll 4
-        for (int p = 0; p < TOKENS / 2; ++p) {
-          const unsigned int r = tok0 + 2 * p + hi;
-          const long long t = (long long)c_now * CHUNK + r;
-          DyVec<T> x;
-          if (DY == DY_RAW) x.load_shared(st + S::RAW, r, l16);
-          else x.load(static_cast<const T *>(a.dy) + t * a.ld, o, t < a.rows ? a.c_out : 0);
-          float v[8];
-          x.get(v);
-          unsigned char *to = st + XB + box + r * 128 + (((l16 & 7) ^ (r & 7)) << 4);
-          uint4 part[PARTS];
-          dw_split<PARTS>(v, part);
-#pragma unroll
-          for (int q = 0; q < PARTS; ++q) *reinterpret_cast<uint4 *>(to + q * DYB) = part[q];
-        }
-      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // visible to the tensor core's reads
       __syncwarp();
-      if (DY == DY_RAW && lane == 0) mbar_arrive(&raw_empty[g]);
       if (lane == 0) mbar_arrive(&conv[g]);
 #pragma unroll
       for (int k = 0; k < EX; ++k) ex[k] = ex_next[k];
@@ -415,7 +378,8 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
         for (int j = 0; j < 16; ++j)
           if (q + j < n) to[(q + j) * stride] = Elem<E>::from_f32(v[j]);
       };
-      const int runs = KEEP32 ? (c1 - c0 + RUN - 1) / RUN : 1;
+      const int low = min(max(a.head - c0, 0), c1 - c0);  // chunks of the smaller parts
+      const int runs = KEEP32 ? (low + kLowRun - 1) / kLowRun + (c1 - c0 - low + a.run - 1) / a.run : 1;
       for (int r = 0; ok && r < runs; ++r) {
         if (!dw_wait(&acc_full[b], aph, abort_v)) { ok = false; break; }
         tc_fence_after();
@@ -555,8 +519,8 @@ __global__ void __launch_bounds__(256)
 // ---- host side ---------------------------------------------------------------------------------------------
 
 struct DwPlan {
-  int bn, i_tiles, o_tiles, chunks, full, segs, units;
-  size_t parts_bytes, bytes;
+  int i_tiles, o_tiles, token_chunks, chunks, full, segs, units;
+  size_t parts_bytes, db_at, split_at, bytes;
 };
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -567,32 +531,39 @@ int db_slices(const dwbnq_affine_desc &d) {
   return (int)(s < 1 ? 1 : s > kDbMaxSlices ? kDbMaxSlices : s);
 }
 
-// `wide`: tiles of 256 output channels. Whole waves of kPlanSms tiles are walked uncut; the R tiles left over are cut into
-// the number of parts that costs least, in chunks on the busiest SM: ceil(R s / SMs) parts of ceil(chunks / s)
-// chunks, each with about 4 chunks' worth of read-back, and 16 for the second kernel and the parts' traffic.
-DwPlan dw_plan(const dwbnq_affine_desc &d, bool wide) {
-  const int chunk = dw_chunk(wide ? DY_TMA : DY_LOAD);
+// bfloat16 parts of dy, and whether they are made in a pass of their own (float16, float32, and bfloat16 rows that TMA cannot take).
+int dw_parts(const dwbnq_affine_desc &d) { return d.dtype == DWBNQ_F32 ? 3 : d.dtype == DWBNQ_F16 ? 2 : 1; }
+bool dw_splits(const dwbnq_affine_desc &d) {
+  return d.dtype != DWBNQ_BF16 || d.dy_unaligned || d.ld_dy % 8 != 0 || d.ld_dy >= (1LL << 36);
+}
+long long dw_pad(const dwbnq_affine_desc &d) { return ((long long)d.c_out + 7) / 8 * 8; }
+
+// Whole waves of kPlanSms tiles are walked uncut; the R tiles left over are cut into the number of parts that costs least, in chunks
+// on the busiest SM: ceil(R s / SMs) parts of ceil(chunks / s) chunks, each with about 4 chunks' worth of read-back, and 8 for the
+// second kernel and the parts' traffic.
+DwPlan dw_plan(const dwbnq_affine_desc &d) {
   DwPlan p;
-  p.bn = wide ? 256 : 128;
   p.i_tiles = (d.c_in + kTileI - 1) / kTileI;
-  p.o_tiles = (d.c_out + p.bn - 1) / p.bn;
-  p.chunks = (int)((d.rows + chunk - 1) / chunk);
+  p.o_tiles = (d.c_out + kBn - 1) / kBn;
+  p.token_chunks = (int)((d.rows + kChunk - 1) / kChunk);
+  p.chunks = p.token_chunks * dw_parts(d);
   const long long tiles = (long long)p.i_tiles * p.o_tiles;
   const int rest = (int)(tiles % kPlanSms);
   p.full = (int)(tiles - rest);
   p.segs = 1;
   long long best = 0;
   for (int s = 1; rest && s <= p.chunks && rest * s <= kMaxParts; ++s) {
-    const long long cost = (long long)((rest * s + kPlanSms - 1) / kPlanSms) * ((p.chunks + s - 1) / s + 4) + (s > 1 ? 16 : 0);
+    const long long cost = (long long)((rest * s + kPlanSms - 1) / kPlanSms) * ((p.chunks + s - 1) / s + 4) + (s > 1 ? 8 : 0);
     if (s == 1 || cost < best) { best = cost; p.segs = s; }
   }
   if (p.segs == 1) p.full = (int)tiles;
   p.units = p.segs == 1 ? (int)tiles : p.full + rest * p.segs;
-  p.parts_bytes = p.segs == 1 ? 0 : up256((size_t)rest * p.segs * p.bn * kTileI * 4);
-  p.bytes = 256 + p.parts_bytes + up256((size_t)db_slices(d) * d.c_out * 4);
+  p.parts_bytes = p.segs == 1 ? 0 : up256((size_t)rest * p.segs * kBn * kTileI * 4);
+  p.db_at = 256 + p.parts_bytes;
+  p.split_at = p.db_at + up256((size_t)db_slices(d) * d.c_out * 4);
+  p.bytes = p.split_at + (dw_splits(d) ? up256((size_t)dw_parts(d) * d.rows * dw_pad(d) * 2) : 0);
   return p;
 }
-bool dw_wide(const dwbnq_affine_desc &d) { return d.dtype == DWBNQ_BF16; }
 
 typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -611,17 +582,28 @@ EncodeFn encode_fn() {
   return fn;
 }
 
-template <typename T, typename TW, int PARTS, int DY, int BN>
+template <typename TW>
 int launch_dw(const CUtensorMap &tm, const CUtensorMap &tc, const DwArgs &a, int dev, cudaStream_t stream) {
-  using S = DwStage<PARTS, BN, DY, (int)sizeof(T)>;
-  const int smem = S::COUNT * S::BYTES + 1024;
-  auto kern = affine_dw_kernel<T, TW, PARTS, DY, BN>;
+  constexpr int smem = kStages * kStageBytes + 1024;
+  auto kern = affine_dw_kernel<TW>;
   static std::atomic<unsigned long long> allowed{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void *>(kern), smem, dev, allowed);
   if (e != cudaSuccess) return fail_cuda(e, "affine_dw_kernel attributes");
   const int sms = sm_count(-1);
   e = launch_pdl(kern, dim3((unsigned)(a.units < sms ? a.units : sms)), dim3(kThreads), (size_t)smem, stream, tm, tc, a);
   return e == cudaSuccess ? DWBNQ_OK : fail_cuda(e, "affine_dw_kernel launch");
+}
+
+template <typename T, int PARTS>
+int launch_split(const dwbnq_affine_desc &d, const void *dy, void *out, cudaStream_t stream) {
+  const OctetGrid g = octet_grid(d.rows, d.c_out, 256, sm_count(-1) * 8);
+  const T *p = static_cast<const T *>(dy);
+  const cudaError_t e = octet_vectors(dy, d.ld_dy, sizeof(T))
+                            ? launch_pdl(affine_split_kernel<T, PARTS, true>, dim3(g.ctas), dim3(256), 0, stream, p, (long long)d.ld_dy,
+                                         (long long)d.rows, d.c_out, g, dw_pad(d), static_cast<uint4 *>(out))
+                            : launch_pdl(affine_split_kernel<T, PARTS, false>, dim3(g.ctas), dim3(256), 0, stream, p, (long long)d.ld_dy,
+                                         (long long)d.rows, d.c_out, g, dw_pad(d), static_cast<uint4 *>(out));
+  return e == cudaSuccess ? DWBNQ_OK : fail_cuda(e, "affine_split_kernel launch");
 }
 
 template <typename T>
@@ -643,61 +625,52 @@ int run_t(const dwbnq_affine_desc &d, const void *codes, const void *exps, const
       return fail_cuda(e, "cudaMemsetAsync");
     return DWBNQ_OK;
   }
-  const int eb = d.dtype == DWBNQ_F32 ? 4 : 2;
-  const bool tma = reinterpret_cast<uintptr_t>(dy) % 16 == 0 && d.ld_dy * eb % 16 == 0 && d.ld_dy < (1LL << 36);
-  const DwPlan p = dw_plan(d, dw_wide(d) && tma);
-  float *parts = reinterpret_cast<float *>(workspace);
-  float *dbp = reinterpret_cast<float *>(static_cast<char *>(workspace) + 256 + p.parts_bytes);
+  const DwPlan p = dw_plan(d);
+  float *parts = reinterpret_cast<float *>(static_cast<char *>(workspace) + 256);
+  float *dbp = reinterpret_cast<float *>(static_cast<char *>(workspace) + p.db_at);
   if (dw) {
     DwArgs a;
     std::memset(&a, 0, sizeof(a));
     a.exps = static_cast<const unsigned char *>(exps);
-    a.dy = dy;
-    a.ld = d.ld_dy; a.rows = d.rows; a.c_in = d.c_in; a.c_out = d.c_out;
+    a.rows = d.rows; a.c_in = d.c_in; a.c_out = d.c_out;
     a.groups = (d.c_in + kCkGroup - 1) / kCkGroup;
-    a.i_tiles = p.i_tiles; a.chunks = p.chunks; a.full = p.full; a.segs = p.segs; a.units = p.units;
+    a.i_tiles = p.i_tiles; a.token_chunks = p.token_chunks; a.chunks = p.chunks; a.full = p.full; a.segs = p.segs; a.units = p.units;
+    a.head = p.chunks - p.token_chunks;
+    a.run = d.dtype == DWBNQ_F32 ? kRunF32 : kRun;
     a.dw = dw; a.parts = parts; a.accum = (accum_mask >> 1) & 1;
     int st = device_flag_ptr(dev, &a.flag);
     if (st != DWBNQ_OK) return st;
-    CUtensorMap tm, tc;
-    std::memset(&tm, 0, sizeof(tm));
-    std::memset(&tc, 0, sizeof(tc));
+    const void *src = dy;
+    long long pitch = d.ld_dy;
+    if (dw_splits(d)) {
+      void *out = static_cast<char *>(workspace) + p.split_at;
+      st = d.dtype == DWBNQ_F32 ? launch_split<float, 3>(d, dy, out, stream)
+           : d.dtype == DWBNQ_F16 ? launch_split<__half, 2>(d, dy, out, stream) : launch_split<__nv_bfloat16, 1>(d, dy, out, stream);
+      if (st != DWBNQ_OK) return st;
+      src = out;
+      pitch = dw_pad(d);
+    }
     if (!encode_fn()) return fail(DWBNQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-    const cuuint32_t es[2] = {1, 1}, chunk = (cuuint32_t)dw_chunk(d.dtype == DWBNQ_BF16 && tma ? DY_TMA : tma ? DY_RAW : DY_LOAD);
+    CUtensorMap tm, tc;
+    const cuuint32_t es[3] = {1, 1, 1};
     const cuuint64_t cdim[2] = {(cuuint64_t)a.groups * kCkGroup, (cuuint64_t)d.rows}, cstr[1] = {cdim[0]};
-    const cuuint32_t cbox[2] = {kTileI, chunk};
+    const cuuint32_t cbox[2] = {kTileI, kChunk};
     CUresult r = encode_fn()(&tc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(codes), cdim, cstr, cbox, es,
                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(DWBNQ_ERR_CUDA, "cuTensorMapEncodeTiled(codes) failed with CUresult %d", (int)r);
-    if (tma) {
-      const cuuint64_t dim[2] = {(cuuint64_t)d.c_out, (cuuint64_t)d.rows}, str[1] = {(cuuint64_t)d.ld_dy * eb};
-      const cuuint32_t box[2] = {(cuuint32_t)(128 / eb), chunk};
-      const bool as_is = d.dtype == DWBNQ_BF16;
-      r = encode_fn()(&tm, as_is ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : eb == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
-                      2, const_cast<void *>(dy), dim, str, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                      as_is ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-      if (r != CUDA_SUCCESS) return fail(DWBNQ_ERR_CUDA, "cuTensorMapEncodeTiled(dy) failed with CUresult %d", (int)r);
-    }
-    if constexpr (sizeof(TW) == 4) {
-      if (d.dtype == DWBNQ_F32)
-        st = tma ? launch_dw<float, TW, 3, DY_RAW, 128>(tm, tc, a, dev, stream) : launch_dw<float, TW, 3, DY_LOAD, 128>(tm, tc, a, dev, stream);
-      else if (d.dtype == DWBNQ_F16)
-        st = tma ? launch_dw<__half, TW, 2, DY_RAW, 128>(tm, tc, a, dev, stream) : launch_dw<__half, TW, 2, DY_LOAD, 128>(tm, tc, a, dev, stream);
-      else
-        st = tma ? launch_dw<__nv_bfloat16, TW, 1, DY_TMA, 256>(tm, tc, a, dev, stream)
-                 : launch_dw<__nv_bfloat16, TW, 1, DY_LOAD, 128>(tm, tc, a, dev, stream);
-    } else if constexpr (std::is_same<TW, __half>::value) {
-      st = tma ? launch_dw<__half, TW, 2, DY_RAW, 128>(tm, tc, a, dev, stream) : launch_dw<__half, TW, 2, DY_LOAD, 128>(tm, tc, a, dev, stream);
-    } else {
-      st = tma ? launch_dw<__nv_bfloat16, TW, 1, DY_TMA, 256>(tm, tc, a, dev, stream)
-               : launch_dw<__nv_bfloat16, TW, 1, DY_LOAD, 128>(tm, tc, a, dev, stream);
-    }
+    const cuuint64_t dim[3] = {(cuuint64_t)d.c_out, (cuuint64_t)d.rows, (cuuint64_t)dw_parts(d)};
+    // a single part has no stride between parts, and rows x ld_dy may be more than one may be
+    const cuuint64_t str[2] = {(cuuint64_t)pitch * 2, (cuuint64_t)pitch * 2 * (dw_splits(d) ? (cuuint64_t)d.rows : 1)};
+    const cuuint32_t box[3] = {64, kChunk, 1};
+    r = encode_fn()(&tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(src), dim, str, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(DWBNQ_ERR_CUDA, "cuTensorMapEncodeTiled(dy) failed with CUresult %d", (int)r);
+    st = launch_dw<TW>(tm, tc, a, dev, stream);
     if (st != DWBNQ_OK) return st;
     if (p.segs > 1) {
-      const dim3 grid((unsigned)((p.units - p.full) / p.segs), (unsigned)(p.bn / 2));
-      e = launch_pdl(affine_dw_join_kernel<TW>, grid, dim3(2 * kTileI), 0, stream, (const float *)parts, p.full, p.segs, p.bn, p.i_tiles,
+      const dim3 grid((unsigned)((p.units - p.full) / p.segs), (unsigned)(kBn / 2));
+      e = launch_pdl(affine_dw_join_kernel<TW>, grid, dim3(2 * kTileI), 0, stream, (const float *)parts, p.full, p.segs, kBn, p.i_tiles,
                      d.c_in, d.c_out, static_cast<TW *>(dw), (accum_mask >> 1) & 1);
       if (e != cudaSuccess) return fail_cuda(e, "affine_dw_join_kernel launch");
     }
@@ -717,10 +690,7 @@ int run_t(const dwbnq_affine_desc &d, const void *codes, const void *exps, const
 
 }  // namespace
 
-size_t affine_bwd_workspace_bytes(const dwbnq_affine_desc &d) {
-  const size_t narrow = dw_plan(d, false).bytes, wide = dw_wide(d) ? dw_plan(d, true).bytes : 0;
-  return narrow > wide ? narrow : wide;
-}
+size_t affine_bwd_workspace_bytes(const dwbnq_affine_desc &d) { return dw_plan(d).bytes; }
 
 int launch_affine_bwd(const dwbnq_affine_desc &d, const void *codes, const void *exps, const void *dy, void *dw, void *db,
                       int accum_mask, void *workspace, int dev, cudaStream_t stream) {

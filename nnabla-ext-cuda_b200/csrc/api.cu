@@ -831,6 +831,8 @@ int dwbnq_affine_bwd_ckpt8(const dwbnq_affine_desc *desc, const void *codes, con
   if (desc->rows > 0) {
     if (!dy) return fail(DWBNQ_ERR_INVALID_ARG, "dy must not be null");
     st = check_elem("dy", dy, desc->dtype);
+    if (st == DWBNQ_OK && !desc->dy_unaligned && reinterpret_cast<uintptr_t>(dy) % 16)
+      return fail(DWBNQ_ERR_INVALID_ARG, "dy is not 16-byte aligned and the desc does not say so (dy_unaligned)");
     if (st == DWBNQ_OK && dw) st = check_ckpt8("checkpoint of x", codes, exps);
   }
   if (st == DWBNQ_OK) st = check_elem("dw", dw, desc->dw_dtype);

@@ -54,7 +54,8 @@ class Code8Desc(ctypes.Structure):
 
 class AffineDesc(ctypes.Structure):
     _fields_ = [("dtype", ctypes.c_int32), ("dw_dtype", ctypes.c_int32), ("rows", ctypes.c_int64),
-                ("c_in", ctypes.c_int32), ("c_out", ctypes.c_int32), ("ld_dy", ctypes.c_int64)]
+                ("c_in", ctypes.c_int32), ("c_out", ctypes.c_int32), ("ld_dy", ctypes.c_int64),
+                ("dy_unaligned", ctypes.c_int32)]
 
 
 class W4Desc(ctypes.Structure):

@@ -292,6 +292,28 @@ def test_affine_gradients_real_values(cuda_device, dt, rows, c_in, c_out):
     assert ((narrow.cpu().double() - want).abs() <= lim).all()
 
 
+@pytest.mark.parametrize("rows,c_in,c_out", [(4300, 1536, 3200), (9001, 64, 96), (20011, 130, 300)])
+@pytest.mark.parametrize("dt", ["f16", "f32"])
+def test_affine_gradients_of_long_batches(cuda_device, dt, rows, c_in, c_out):
+    """dy in several bfloat16 parts over more tokens than a run of the lower parts, in whole tiles and in tiles cut anywhere."""
+    dtype = fb.TYPES[dt]
+    x, dy = (t.to(cuda_device) for t in dw_case(rows, c_in, c_out, dtype, 37, False))
+    dy[:, 0] = 1 + dy[:, 0].abs() / 16  # one sign and every digit in use
+    ck = ops.checkpoint_code8(x)
+    xv = ops.restore_code8(ck, torch.float32).double()
+    want, size = dy.double().T @ xv, dy.double().abs().T @ xv.abs()
+    dw, _ = ops.affine_weight_backward(ck, dy, need=(True, False), dtype=torch.float32)
+    # the bounds of the shorter batches
+    assert ((dw.double() - want).abs() <= (rows + 8) * 2.0 ** -23 * size).all()
+    assert (dw.double() - want).norm() <= 1.5e-6 * want.norm()
+    base = torch.randn(c_out, c_in, generator=gen(4)).to(cuda_device)
+    acc, _ = ops.affine_weight_backward(ck, dy, dw=base.clone(), need=(True, False), accum=(True, False))
+    # one addition more per run: a run has at least 512 tokens
+    assert ((acc.double() - base.double() - want).abs() <= (rows + 8) * 2.0 ** -23 * size + (rows / 512 + 2) * 2.0 ** -24 * base.abs()).all()
+    assert torch.equal(ops.affine_weight_backward(ck, dy, need=(True, False), dtype=torch.float32)[0], dw)
+    ops.check_device_flag()
+
+
 def test_affine_gradients_of_nothing(cuda_device):
     ck = ops.checkpoint_code8(torch.empty(0, 40, device=cuda_device))
     dy = torch.empty(0, 24, device=cuda_device)

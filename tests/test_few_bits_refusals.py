@@ -81,6 +81,19 @@ def test_affine_backward_refusals():
     assert lib.dwbnq_affine_bwd_workspace_bytes(ctypes.byref(desc())) > 0
 
 
+def test_affine_backward_unaligned_dy_is_declared():
+    """A dy off the 16-byte grid needs a workspace that only a descriptor which says so is given."""
+    def desc(**kw):
+        return L.AffineDesc(**dict(dict(dtype=L.BF16, dw_dtype=L.F32, rows=640, c_in=40, c_out=24, ld_dy=24), **kw))
+
+    size = lambda **kw: L.lib().dwbnq_affine_bwd_workspace_bytes(ctypes.byref(desc(**kw)))  # noqa: E731
+    st, msg = call("dwbnq_affine_bwd_ckpt8", ctypes.byref(desc()), P, P, P + 2, P, P, 0, P, -1, None)
+    assert st == L.ERR_INVALID_ARG and "dy_unaligned" in msg
+    assert size(dy_unaligned=1) == size() + 640 * 24 * 2 and size(ld_dy=25) == size(dy_unaligned=1)
+    # three parts, and 30 chunks of 64 tokens instead of 10, each with a tile of 128 x 256 sums
+    assert size(dtype=L.F32) == size() + 3 * 640 * 24 * 2 + (30 - 10) * 128 * 256 * 4
+
+
 def test_w4_refusals():
     def desc(**kw):
         return L.W4Desc(**dict(dict(dtype=L.BF16, group=64, c_in=128, c_out=24, has_zeros=0), **kw))
