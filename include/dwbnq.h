@@ -451,7 +451,7 @@ typedef struct dwbnq_affine_desc {
  * entry; calls that may overlap on the GPU need one each. 0 for an invalid descriptor. Small for
  * DWBNQ_BF16 with rows that start on 16-byte boundaries (ld_dy a multiple of 8, dy_unaligned 0);
  * otherwise dy is first laid out as bfloat16 parts there: 2, 4 or 6 bytes per element of dy for
- * DWBNQ_BF16, _F16 and _F32. */
+ * DWBNQ_BF16, _F16 and _F32 (c_in 0, as a call for db alone may say, needs no such scratch). */
 size_t dwbnq_affine_bwd_workspace_bytes(const dwbnq_affine_desc *desc);
 /* Weight and bias gradients with the input read from its checkpoint (codes and exps of x [rows,
  * c_in]): dw[o][i] (+)= sum over rows of dy[r][o] * x[r][i], dw [c_out, c_in] contiguous;

@@ -417,29 +417,40 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
   }
 }
 
-// dw of the tiles whose tokens were cut into `segs` parts: the parts added in order, eight of them in flight. CTA = tile x two of
-// its columns.
-template <typename TW>
+// dw of the tiles whose tokens were cut into `segs` parts: the parts added in order. CTA = tile x 2 COLS of its columns; a thread has
+// COLS columns and 8 or 16 loads in flight. With many tiles of few parts, four columns per thread are fewer CTAs to start (40 tiles
+// of three parts, fp32: 6.5 against 9.0 us); with few tiles one per thread keeps the SMs busy.
+template <typename TW, int COLS>
 __global__ void __launch_bounds__(2 * kTileI)
     affine_dw_join_kernel(const float *__restrict__ parts, int first_tile, int segs, int bn, int i_tiles, int c_in, int c_out,
                           TW *__restrict__ dw, int accum) {
+  constexpr int AHEAD = COLS == 1 ? 8 : 4;
   pdl_launch_dependents();
   pdl_wait_for_predecessor();
-  const int tile = first_tile + blockIdx.x, ot = tile / i_tiles, il = threadIdx.x % kTileI, n = blockIdx.y * 2 + threadIdx.x / kTileI;
+  const int tile = first_tile + blockIdx.x, ot = tile / i_tiles, il = threadIdx.x % kTileI;
+  const int n = blockIdx.y * 2 * COLS + threadIdx.x / kTileI;  // and every second one after it
   const int i = (tile - ot * i_tiles) * kTileI + il, o = ot * bn + n;
   if (i >= c_in || o >= c_out) return;
   const float *p = parts + ((long long)blockIdx.x * segs * bn + n) * kTileI + il;
   const long long step = (long long)bn * kTileI;
-  float s = 0.0f;
-  for (int k = 0; k < segs; k += 8) {
-    float v[8];
+  float s[COLS] = {};
+  for (int k = 0; k < segs; k += AHEAD) {
+    float v[AHEAD][COLS];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = k + j < segs ? p[(k + j) * step] : 0.0f;
+    for (int j = 0; j < AHEAD; ++j)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s = __fadd_rn(s, v[j]);
+      for (int c = 0; c < COLS; ++c) v[j][c] = k + j < segs && o + 2 * c < c_out ? p[(k + j) * step + 2 * c * kTileI] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) s[c] = __fadd_rn(s[c], v[j][c]);
   }
-  TW *q = dw + (long long)o * c_in + i;
-  *q = Elem<TW>::from_f32(accum ? __fadd_rn(Elem<TW>::to_f32(*q), s) : s);
+#pragma unroll
+  for (int c = 0; c < COLS; ++c) {
+    if (o + 2 * c >= c_out) break;
+    TW *q = dw + (long long)(o + 2 * c) * c_in + i;
+    *q = Elem<TW>::from_f32(accum ? __fadd_rn(Elem<TW>::to_f32(*q), s[c]) : s[c]);
+  }
 }
 
 // ---- bias gradient: CTA (64 channels, slice of the rows), a lane two channels, warp w the rows w, w + 8, ..., eight of them in
@@ -561,7 +572,7 @@ DwPlan dw_plan(const dwbnq_affine_desc &d) {
   p.parts_bytes = p.segs == 1 ? 0 : up256((size_t)rest * p.segs * kBn * kTileI * 4);
   p.db_at = 256 + p.parts_bytes;
   p.split_at = p.db_at + up256((size_t)db_slices(d) * d.c_out * 4);
-  p.bytes = p.split_at + (dw_splits(d) ? up256((size_t)dw_parts(d) * d.rows * dw_pad(d) * 2) : 0);
+  p.bytes = p.split_at + (dw_splits(d) && d.c_in ? up256((size_t)dw_parts(d) * d.rows * dw_pad(d) * 2) : 0);
   return p;
 }
 
@@ -669,9 +680,11 @@ int run_t(const dwbnq_affine_desc &d, const void *codes, const void *exps, const
     st = launch_dw<TW>(tm, tc, a, dev, stream);
     if (st != DWBNQ_OK) return st;
     if (p.segs > 1) {
-      const dim3 grid((unsigned)((p.units - p.full) / p.segs), (unsigned)(kBn / 2));
-      e = launch_pdl(affine_dw_join_kernel<TW>, grid, dim3(2 * kTileI), 0, stream, (const float *)parts, p.full, p.segs, kBn, p.i_tiles,
-                     d.c_in, d.c_out, static_cast<TW *>(dw), (accum_mask >> 1) & 1);
+      const int cut = (p.units - p.full) / p.segs;
+      const bool many = cut * (kBn / 2) > 16 * kPlanSms;  // more than two waves of CTAs
+      e = launch_pdl(many ? affine_dw_join_kernel<TW, 4> : affine_dw_join_kernel<TW, 1>, dim3((unsigned)cut, (unsigned)(kBn / (many ? 8 : 2))),
+                     dim3(2 * kTileI), 0, stream, (const float *)parts, p.full, p.segs, kBn, p.i_tiles, d.c_in, d.c_out,
+                     static_cast<TW *>(dw), (accum_mask >> 1) & 1);
       if (e != cudaSuccess) return fail_cuda(e, "affine_dw_join_kernel launch");
     }
   }

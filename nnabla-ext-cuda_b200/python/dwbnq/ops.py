@@ -548,7 +548,8 @@ def affine_weight_backward(ck_x, dy, dw=None, db=None, need=(True, True), accum=
         if t is not None and not t.is_contiguous():
             raise ValueError("%s must be contiguous" % n)
     dev = _one_device(dy, ck_x.codes, ck_x.exponents, dw, db, ws)
-    d = L.AffineDesc(dtype=code, dw_dtype=_few_bits_code(dtype), rows=rows, c_in=c_in, c_out=c_out, ld_dy=ld,
+    # without dw nothing of x is read, and no scratch is needed for the parts of dy
+    d = L.AffineDesc(dtype=code, dw_dtype=_few_bits_code(dtype), rows=rows, c_in=c_in if need[0] else 0, c_out=c_out, ld_dy=ld,
                      dy_unaligned=int(dy.data_ptr() % 16 != 0))
     mask = (2 if accum[0] else 0) | (4 if accum[1] else 0)
     if ws is None:

@@ -90,6 +90,7 @@ def test_affine_backward_unaligned_dy_is_declared():
     st, msg = call("dwbnq_affine_bwd_ckpt8", ctypes.byref(desc()), P, P, P + 2, P, P, 0, P, -1, None)
     assert st == L.ERR_INVALID_ARG and "dy_unaligned" in msg
     assert size(dy_unaligned=1) == size() + 640 * 24 * 2 and size(ld_dy=25) == size(dy_unaligned=1)
+    assert size(dtype=L.F32, c_in=0) < 10000  # db alone
     # three parts, and 30 chunks of 64 tokens instead of 10, each with a tile of 128 x 256 sums
     assert size(dtype=L.F32) == size() + 3 * 640 * 24 * 2 + (30 - 10) * 128 * 256 * 4
 
