@@ -1,4 +1,4 @@
-"""Plain 64-bit implementations of the affine layer in few bits (checker of the tests, NumPy / torch on the CPU)."""
+"""Plain 64-bit implementations of the affine layer in few bits (the oracle of the tests, NumPy / torch on the CPU)."""
 import math
 
 import numpy as np
