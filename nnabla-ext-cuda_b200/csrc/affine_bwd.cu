@@ -10,16 +10,17 @@
 //    accumulator back holds 32 consecutive elements of one row of dw per column, so every store is a
 //    coalesced line and nothing is staged. Both factors are MN-major in shared memory, as they lie in
 //    global memory: no transpose anywhere;
-//  * per CTA (one per SM): warp 0 issues the TMA loads, warp 1 the MMAs, warps 2-17 expand the codes into the
-//    swizzled operand layout, warps 18-25 read the accumulators back. The converters work in as many groups as
+//  * per CTA (one per SM): warps 0-15 expand the codes into the swizzled operand layout, warps 16-23 read the accumulators back,
+//    warp 24 issues the TMA loads, warp 25 the MMAs, warps 26 and 27 bring the exponents. The converters work in as many groups as
 //    there are stages, a chunk of 64 tokens per group: one warp needs about 1400 cycles from its wait to its next
 //    one, and with all of them on every chunk that was the kernel's pace (512 cycles of MMAs per chunk);
-//  * where the result is kept in 32 bits, the accumulator is read back after a run of a few chunks and the runs
-//    are added to dw in fp32: the tensor core's adder truncates, by 2^-25 of the sum per step of 16 tokens on
-//    average, and over a long batch that would be the result's error;
+//  * the tensor core's adder truncates, by 2^-25 of the sum per step of 16 tokens on average and up to 2^-23. Left alone over 65536
+//    tokens that was half a rounding step of float16. So every sum is cut into runs of 512 tokens, which are added in fp32: the
+//    accumulators are double, and while one takes the next run the epilogue adds the other's to sums that it keeps in
+//    registers (128 columns per lane) until the unit is done. Adding the runs to dw in memory instead cost a quarter of the time;
 //  * what bounds it: the way of a stage - copy 1600 cycles, expansion 800, issue and MMAs 1000 - against the four stages that fit;
-//    8192 tokens, 4096 x 4096, bf16: 256 us, 1072 TFLOP/s (322 us with a 32-bit result; fp16 509 us, two products; fp32 1026 us,
-//    three products, and 4 GB of partial results through L2);
+//    8192 tokens, 4096 x 4096, inputs in L2 from the call before: bf16 254 us, 1080 TFLOP/s, with a 32-bit result 259; fp16
+//    511 us, two products; fp32 786 us, three;
 //  * tiles that fill whole waves of the 148 SMs are walked as they are; the tiles of the last, partial wave
 //    are cut along the tokens so that it is full too, and a second kernel adds their parts in a fixed order.
 #include <cstring>
@@ -34,11 +35,19 @@ namespace {
 
 constexpr int kTileI = 128;       // input channels per tile = TMEM lanes
 constexpr int kChunk = 64;        // tokens per pipeline stage
-// Chunks per run of a result kept in 32 bits. What the adder drops is relative to the sum, so the parts of dy below the leading
-// digits (at most 2^-7 of it) may run longer; a float32 dy is held to half of what 16 bits are.
-constexpr int kRun = 16, kRunF32 = 8, kLowRun = 64;
-constexpr int kConvWarps = 16, kFirstEpi = 2 + kConvWarps, kEpiWarps = 8;
-constexpr int kThreads = 32 * (kFirstEpi + kEpiWarps);
+// Chunks per run. What the adder drops is relative to the sum, so the parts of dy below the leading digits (at most 2^-7 of it) may
+// run longer. A run costs 128 loads and additions per epilogue lane, beside the MMAs of the next one: runs of 8, 16, 32 chunks and of
+// the whole batch take the same time within 1% (8192 tokens, 4096 x 4096 bf16).
+constexpr int kRun = 8, kLowRun = 64;
+constexpr int kConvWarps = 16, kEpiWarps = 8, kTmaWarp = kConvWarps + kEpiWarps, kMmaWarp = kTmaWarp + 1, kExpWarp = kTmaWarp + 2;
+constexpr int kThreads = 32 * (kConvWarps + kEpiWarps + 4);
+// Registers per thread. The epilogue's sums want twice what a block of this size may be launched with, so the groups of four warps set
+// their own number; together they are what the launch was given. (Converters with 40 and an epilogue with 136 that spills: 262 us;
+// converters that load exponents themselves, with 48: 262; issuers with 40 or 24: 263 and 271.)
+constexpr int kRegsLaunch = 72, kRegsConv = 32, kRegsEpi = 152, kRegsIssue = 72;
+static_assert(kThreads * kRegsLaunch <= 65536 && kConvWarps % 4 == 0 && kEpiWarps % 4 == 0 &&
+                  kConvWarps * kRegsConv + kEpiWarps * kRegsEpi + 4 * kRegsIssue <= kThreads / 32 * kRegsLaunch,
+              "a warp that asks for more registers than the others gave back would wait for good");
 constexpr int kTmemCols = 512;
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kPlanSms = 148;     // SMs of a B200: the cut of the last wave does not depend on the device it is asked on
@@ -52,7 +61,7 @@ struct DwArgs {
   int token_chunks;        // ceil(rows / 64)
   int chunks;              // of a tile: token_chunks of every bfloat16 part of dy, the smallest part first
   int head;                // the first chunk of the part that holds dy's leading digits
-  int run;                 // chunks per run there
+  int exps_words;          // every row of exponents starts on a 4-byte boundary
   int full, segs, units;   // units 0 .. full-1: whole tiles; then segs parts of every further tile
   void *dw;
   float *parts;            // [unit - full][tile columns][128]
@@ -154,7 +163,8 @@ __global__ void __launch_bounds__(256)
 // always awaited by the same group (a parity wait cannot tell a phase from the one after the next).
 constexpr int kBn = 256, kXBytes = kChunk * kTileI * 2, kDyBytes = kChunk * kBn * 2, kStageBytes = kXBytes + kDyBytes + kChunk * kTileI;
 constexpr int kStages = 4, kBox = kChunk * 128;  // a box: 64 tokens x 128 bytes
-static_assert(kStageBytes % 1024 == 0 && kStages * kStageBytes + 2048 <= kSmemMax, "swizzle atoms; shared memory");
+constexpr int kTileGroups = kTileI / kCkGroup, kExpBytes = kChunk * kTileGroups;  // exponents of a stage
+static_assert(kStageBytes % 1024 == 0 && kStages * (kStageBytes + kExpBytes) + 1536 <= kSmemMax, "swizzle atoms; shared memory");
 
 // pw_wait for a warp of a CTA that may be giving up: the flag is looked at only when the barrier is not ready.
 __device__ __forceinline__ bool dw_wait(unsigned long long *bar, unsigned int parity, volatile int *abort_v) {
@@ -162,16 +172,24 @@ __device__ __forceinline__ bool dw_wait(unsigned long long *bar, unsigned int pa
   return pw_wait(bar, parity) && !*abort_v;
 }
 
-// TW: type of dw (32 bits: sums in short runs).
+// The pointer, in a way the compiler cannot compute ahead of: all columns' addresses at once would not fit the registers.
+template <typename T> __device__ __forceinline__ T *after(T *p) {
+  asm volatile("" : "+l"(p));
+  return p;
+}
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// TW: type of dw.
 template <typename TW>
 __global__ void __launch_bounds__(kThreads, 1)
 affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ CUtensorMap tm_codes, const DwArgs a) {
   constexpr int BN = kBn, GROUP = kConvWarps / kStages, TOKENS = kChunk / GROUP;  // converter warps per group, tokens per warp and chunk
-  constexpr bool KEEP32 = sizeof(TW) == 4;
   constexpr int NACC = kTmemCols / BN;
   constexpr int HALF = BN / 2;                        // columns per epilogue warp
   extern __shared__ unsigned char smem_raw[];
   __shared__ unsigned long long bars[3 * kStages + 2 * NACC + 1];
+  __shared__ __align__(16) unsigned char exps_s[kStages][kExpBytes];  // [token][group of channels]
   __shared__ unsigned int tmem_base_s;
   __shared__ int abort_s;
   unsigned long long *full = bars, *empty = bars + kStages, *conv = bars + 2 * kStages;
@@ -182,7 +200,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], 2);  // the copies' and the exponents'
       mbar_init(&empty[s], 1);
       mbar_init(&conv[s], GROUP);
     }
@@ -194,7 +212,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
     abort_s = 0;
     mbar_fence_init();
   }
-  if (warp == 1) {
+  if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)),
                  "r"(kTmemCols)
                  : "memory");
@@ -207,8 +225,14 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
   pdl_wait_for_predecessor();
   const unsigned int tmem_base = tmem_base_s;
   volatile int *abort_v = &abort_s;
+  int total = 0;  // chunks of this CTA
+  for (int u = blockIdx.x; u < a.units; u += gridDim.x) {
+    int tile, c0, c1;
+    dw_unit(a, u, tile, c0, c1);
+    total += c1 - c0;
+  }
 
-  if (warp == 0) {
+  if (warp == kTmaWarp) {
     // ---- TMA loads, boxes of 64 tokens x 128 bytes, zero beyond the tensors: the codes, and dy or one of its parts ----
     int s = 0, issued = 0;
     unsigned int ph = 0;
@@ -243,7 +267,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
         pw_wait_lane(&full[s], ph);
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == kMmaWarp) {
     // ---- MMAs: the warp walks through the chunks, one elected lane issues ----
     // fp32 accumulator, bfloat16 factors, both MN-major, M = 128; N is set per tile
     const unsigned int idesc0 = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | (8u << 24);
@@ -263,7 +287,7 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
         // dy and the codes of the stage have landed when its converters have arrived: they waited for them
         if ((run == 0 && !dw_wait(&acc_empty[b], aph ^ 1u, abort_v)) || !dw_wait(&conv[s], ph, abort_v)) { ok = false; break; }
         tc_fence_after();
-        const bool last = c == c1 - 1 || (KEEP32 && (run == (c < a.head ? kLowRun : a.run) - 1 || c == a.head - 1));
+        const bool last = c == c1 - 1 || run == (c < a.head ? kLowRun : kRun) - 1 || c == a.head - 1;
         const int steps = ++ct == a.token_chunks ? last_steps : kChunk / 16;
         const unsigned long long so = (unsigned long long)(s * kStageBytes) >> 4, dx = dx0 + so, dd = dd0 + so;
         const unsigned int d = tmem_base + b * BN;
@@ -290,129 +314,164 @@ affine_dw_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constan
       __syncwarp();
       pw_wait(drained, 0);
     }
-  } else if (warp < kFirstEpi) {
-    // ---- converters: group g has the chunks n = g, g + kStages, ... of this CTA and with them stage g; a warp has TOKENS tokens
-    // of the chunk, a pass is two tokens, a lane eight channels. The exponents of a warp's tokens come by byte loads, one chunk
-    // of the group ahead. The code is kept short: unrolled over several chunks it threw the instructions of the warps that
-    // issue the loads and the MMAs out of the instruction cache ----
-    const int g = (warp - 2) / GROUP, l16 = lane & 15, hi = lane >> 4;
-    const unsigned int tok0 = ((warp - 2) % GROUP) * TOKENS, box = (l16 >> 3) * (unsigned)kBox;
-    unsigned char *st = sm + g * kStageBytes;
-    static_assert(TOKENS >= 8, "a byte of exponents for every lane");
-    constexpr int EX = TOKENS * 4 / 32;  // exponents per lane: four groups of 32 channels per token
-    int u = blockIdx.x, tile = 0, c = 0, c1 = 0;
-    // the cursor moves `by` chunks on, into the next units where need be
-    auto move = [&](int by) {
-      c += by;
-      while (u < a.units && c >= c1) {
-        int c0;
-        const int over = c - c1;
-        u += gridDim.x;
-        if (u < a.units) {
-          dw_unit(a, u, tile, c0, c1);
-          c = c0 + over;
+  } else if (warp >= kExpWarp) {
+    // ---- exponents: two warps, every other chunk each, one chunk of the warp's ahead. Four groups of a token are one word where every
+    // row of them starts on a word; else they come by byte loads ----
+    const bool words = a.exps_words;
+    int u = blockIdx.x, left = 0, ct = 0, gr = 0;  // chunks left of the unit, this one's number in its part of dy, the lane's group of channels
+    // the cursor comes to the chunk `over` behind the start of unit u, which may lie in a later unit
+    auto enter = [&](int over) {
+      for (; u < a.units; u += gridDim.x) {
+        int tile, c0, c1;
+        dw_unit(a, u, tile, c0, c1);
+        left = c1 - c0 - over;
+        if (left > 0) {
+          ct = (c0 + over) % a.token_chunks;
+          gr = tile % a.i_tiles * kTileGroups + (words ? 0 : lane & 3);
+          return;
         }
+        over = -left;
       }
     };
-    auto exponents = [&](unsigned int(&e)[EX]) {
-      const int gr = tile % a.i_tiles * (kTileI / kCkGroup) + (lane & 3);
+    auto take = [&](unsigned int(&e)[8]) {  // those of the cursor's chunk; the cursor moves on
+      unsigned int t = (unsigned)ct * kChunk + (words ? lane : lane >> 2);  // below 2^31
+      const unsigned char *p = a.exps + (unsigned long long)t * (unsigned)a.groups + gr;
+      const bool in = u < a.units && gr < a.groups;
+      if (words) {
 #pragma unroll
-      for (int k = 0; k < EX; ++k) {
-        const long long t = (long long)(c % a.token_chunks) * kChunk + tok0 + k * 8 + (lane >> 2);
-        e[k] = u < a.units && t < a.rows && gr < a.groups ? __ldg(a.exps + t * a.groups + gr) : kCkMinExp;
+        for (int k = 0; k < 2; ++k, t += 32, p += 32LL * a.groups)
+          e[k] = in && t < a.rows ? __ldg(reinterpret_cast<const unsigned int *>(p)) : kCkMinExp * 0x01010101u;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k, t += 8, p += 8LL * a.groups) e[k] = in && t < a.rows ? __ldg(p) : kCkMinExp;
+      }
+      left -= 2;
+      ct += 2;
+      if (left <= 0) {
+        u += gridDim.x;
+        enter(-left);
+      } else {
+        while (ct >= a.token_chunks) ct -= a.token_chunks;
       }
     };
-    const unsigned int magic = opaque_constant(0x43004300u);
-    unsigned int ex[EX], ex_next[EX], ph = 0;
-    if (u < a.units) dw_unit(a, u, tile, c, c1);
-    move(g);
-    exponents(ex);
+    unsigned int e[8], next[8], ph = 0;
     bool ok = true;
-    while (u < a.units) {
-      move(kStages);
-      exponents(ex_next);
+    enter(warp - kExpWarp);
+    take(e);
+    int s = warp - kExpWarp;
+    for (int n = s; n < total; n += 2) {
+      take(next);
+      if (!dw_wait(&empty[s], ph ^ 1u, abort_v)) { ok = false; break; }
+      if (words) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) reinterpret_cast<unsigned int *>(exps_s[s])[k * 32 + lane] = e[k];
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) exps_s[s][k * 32 + lane] = (unsigned char)e[k];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) e[k] = next[k];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[s]);
+      s += 2;
+      if (s >= kStages) { s -= kStages; ph ^= 1u; }
+    }
+    if (!ok && lane == 0 && !*abort_v) { atomicExch(a.flag, 1); *abort_v = 1; }
+  } else if (warp < kConvWarps) {
+    // ---- converters: group g has the chunks n = g, g + kStages, ... of this CTA and with them stage g; a warp has TOKENS tokens
+    // of the chunk, a pass is two tokens, a lane eight channels. The code is kept short: unrolled over several chunks it threw
+    // the instructions of the warps that issue the loads and the MMAs out of the instruction cache ----
+    fewer_registers<kRegsConv>();
+    const int g = warp / GROUP, l16 = lane & 15, hi = lane >> 4;
+    const unsigned int tok0 = (warp % GROUP) * TOKENS, box = (l16 >> 3) * (unsigned)kBox;
+    unsigned char *st = sm + g * kStageBytes;
+    const unsigned int magic = opaque_constant(0x43004300u);
+    unsigned int ph = 0;
+    bool ok = true;
+    for (int n = g; n < total; n += kStages) {
       if (!dw_wait(&full[g], ph, abort_v)) { ok = false; break; }
 #pragma unroll
       for (int p = 0; p < TOKENS / 2; ++p) {
-        const unsigned int r = tok0 + 2 * p + hi;
+        const unsigned int r = tok0 + 2 * p + hi, e = exps_s[g][r * kTileGroups + (l16 >> 2)];
         const uint2 code = *reinterpret_cast<const uint2 *>(st + kXBytes + kDyBytes + r * kTileI + l16 * 8);
-        const unsigned int e = __shfl_sync(0xffffffffu, ex[p / 4], (2 * (p & 3) + hi) * 4 + (l16 >> 2));
         *reinterpret_cast<uint4 *>(st + box + r * 128 + (((l16 & 7) ^ (r & 7)) << 4)) = dw_expand(code, e, magic);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // visible to the tensor core's reads
       __syncwarp();
       if (lane == 0) mbar_arrive(&conv[g]);
-#pragma unroll
-      for (int k = 0; k < EX; ++k) ex[k] = ex_next[k];
       ph ^= 1u;
     }
     if (!ok && lane == 0 && !*abort_v) { atomicExch(a.flag, 1); *abort_v = 1; }
-  } else {
-    // ---- epilogue: warp (half, quarter) owns input channels [32 quarter, +32) and half of the columns ----
-    const int quarter = warp & 3, half = (warp - kFirstEpi) >> 2;
+  } else if (warp < kTmaWarp) {
+    // ---- epilogue: warp (half, quarter) owns input channels [32 quarter, +32) and half of the columns. A lane keeps its columns'
+    // sums in registers while the runs of a unit come in, and stores them once ----
+    more_registers<kRegsEpi>();
+    const int quarter = warp & 3, half = (warp - kConvWarps) >> 2;
     int b = 0;
     unsigned int aph = 0;
     bool ok = true;
     for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
       int tile, c0, c1;
       dw_unit(a, u, tile, c0, c1);
-      const int ot = tile / a.i_tiles, il = quarter * 32 + lane, i = (tile - ot * a.i_tiles) * kTileI + il;
-      const int o0 = ot * BN + half * HALF, n = min(HALF, a.c_out - o0);  // columns that exist (may be negative)
-      const bool whole = u < a.full;
-      TW *dw = static_cast<TW *>(a.dw) + (long long)o0 * a.c_in + i;
-      float *part = whole ? nullptr : a.parts + ((long long)(u - a.full) * BN + half * HALF) * kTileI + il;
-      const bool i_ok = i < a.c_in;
-      // Run r of the unit: the first is stored (or added to what is there, where the caller accumulates), the others are added.
-      // The sixteen loads go out together, before any of the sums is stored.
-      auto add_to = [&](auto *to, long long stride, int q, float *v) {
-        using E = std::remove_pointer_t<decltype(to)>;
-        E old[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) old[j] = q + j < n ? to[(q + j) * stride] : Elem<E>::from_f32(0.0f);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = __fadd_rn(Elem<E>::to_f32(old[j]), v[j]);
-      };
-      auto put = [&](auto *to, long long stride, int q, const float *v) {
-        using E = std::remove_pointer_t<decltype(to)>;
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (q + j < n) to[(q + j) * stride] = Elem<E>::from_f32(v[j]);
-      };
+      const int ot = tile / a.i_tiles, o0 = ot * BN + half * HALF, n = min(HALF, a.c_out - o0);  // columns that exist (may be negative)
       const int low = min(max(a.head - c0, 0), c1 - c0);  // chunks of the smaller parts
-      const int runs = KEEP32 ? (low + kLowRun - 1) / kLowRun + (c1 - c0 - low + a.run - 1) / a.run : 1;
-      for (int r = 0; ok && r < runs; ++r) {
+      float sum[HALF];
+#pragma unroll
+      for (int j = 0; j < HALF; ++j) sum[j] = 0.0f;
+      for (int r = (low + kLowRun - 1) / kLowRun + (c1 - c0 - low + kRun - 1) / kRun; r > 0; --r) {
         if (!dw_wait(&acc_full[b], aph, abort_v)) { ok = false; break; }
         tc_fence_after();
         const unsigned int taddr = tmem_base + ((unsigned)(quarter * 32) << 16) + b * BN + half * HALF;
-#pragma unroll 1
-        for (int q = 0; q < HALF && q < n; q += 16) {
-          unsigned int acc[2][8];
-          tc_ld8(taddr + q, acc[0]);
-          tc_ld8(taddr + q + 8, acc[1]);
-          tc_ld_wait8(acc[0]);
-          tc_ld_wait8(acc[1]);
-          float v[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(acc[j >> 3][j & 7]);
-          if (!whole) {
-            if (r) add_to(part, kTileI, q, v);
-            put(part, kTileI, q, v);
-          } else if (i_ok) {
-            if (r || a.accum) add_to(dw, a.c_in, q, v);
-            put(dw, a.c_in, q, v);
+        for (int q = 0; q < HALF; q += 8)
+          if (q < n) {
+            unsigned int acc[8];
+            tc_ld8(taddr + q, acc);
+            tc_ld_wait8(acc);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[q + j] = __fadd_rn(sum[q + j], __uint_as_float(acc[j]));
           }
-        }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&acc_empty[b]);
         if (++b == NACC) { b = 0; aph ^= 1u; }
+      }
+      if (!ok) break;
+      const int il = quarter * 32 + lane, i = (tile - ot * a.i_tiles) * kTileI + il;
+      if (u >= a.full) {
+        float *part = a.parts + ((long long)(u - a.full) * BN + half * HALF) * kTileI + il;
+#pragma unroll
+        for (int q = 0; q < HALF; q += 8) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (q + j < n) part[j * kTileI] = sum[q + j];
+          part = after(part + 8 * kTileI);
+        }
+      } else if (i < a.c_in) {
+        TW *dw = static_cast<TW *>(a.dw) + (long long)o0 * a.c_in + i;
+#pragma unroll
+        for (int q = 0; q < HALF; q += 8) {
+          TW *to = dw;
+          if (a.accum) {  // eight loads go out together
+            TW old[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j, to += a.c_in) old[j] = q + j < n ? *to : Elem<TW>::from_f32(0.0f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[q + j] = __fadd_rn(Elem<TW>::to_f32(old[j]), sum[q + j]);
+            to = dw;
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j, to += a.c_in)
+            if (q + j < n) *to = Elem<TW>::from_f32(sum[q + j]);
+          dw = after(to);
+        }
       }
     }
     if (!ok && lane == 0 && !*abort_v) { atomicExch(a.flag, 1); *abort_v = 1; }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (warp == kMmaWarp) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
   }
 }
@@ -598,7 +657,13 @@ int launch_dw(const CUtensorMap &tm, const CUtensorMap &tc, const DwArgs &a, int
   constexpr int smem = kStages * kStageBytes + 1024;
   auto kern = affine_dw_kernel<TW>;
   static std::atomic<unsigned long long> allowed{0};
-  cudaError_t e = allow_smem(reinterpret_cast<const void *>(kern), smem, dev, allowed);
+  cudaError_t e;
+  if (!allowed.load(std::memory_order_acquire)) {  // the split of the registers counts on what the kernel was compiled to
+    cudaFuncAttributes fa;
+    if ((e = cudaFuncGetAttributes(&fa, kern)) != cudaSuccess) return fail_cuda(e, "affine_dw_kernel attributes");
+    if (fa.numRegs != kRegsLaunch) return fail(DWBNQ_ERR_UNSUPPORTED, "affine_dw_kernel was built with %d registers", fa.numRegs);
+  }
+  e = allow_smem(reinterpret_cast<const void *>(kern), smem, dev, allowed);
   if (e != cudaSuccess) return fail_cuda(e, "affine_dw_kernel attributes");
   const int sms = sm_count(-1);
   e = launch_pdl(kern, dim3((unsigned)(a.units < sms ? a.units : sms)), dim3(kThreads), (size_t)smem, stream, tm, tc, a);
@@ -645,9 +710,9 @@ int run_t(const dwbnq_affine_desc &d, const void *codes, const void *exps, const
     a.exps = static_cast<const unsigned char *>(exps);
     a.rows = d.rows; a.c_in = d.c_in; a.c_out = d.c_out;
     a.groups = (d.c_in + kCkGroup - 1) / kCkGroup;
+    a.exps_words = (reinterpret_cast<uintptr_t>(exps) | a.groups) % 4 == 0;
     a.i_tiles = p.i_tiles; a.token_chunks = p.token_chunks; a.chunks = p.chunks; a.full = p.full; a.segs = p.segs; a.units = p.units;
     a.head = p.chunks - p.token_chunks;
-    a.run = d.dtype == DWBNQ_F32 ? kRunF32 : kRun;
     a.dw = dw; a.parts = parts; a.accum = (accum_mask >> 1) & 1;
     int st = device_flag_ptr(dev, &a.flag);
     if (st != DWBNQ_OK) return st;
