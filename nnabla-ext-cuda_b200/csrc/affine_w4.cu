@@ -93,24 +93,24 @@ __global__ void __launch_bounds__(256)
 // one row of x costs what eight cost, and for a handful the kernel is bound by reading the weights, 4 bits each. tcgen05 would want
 // 128 output channels per tile and the weights in shared or tensor memory; here they go from global memory to the
 // instruction through registers only. A lane's word of eight codes is the A operand of two instructions: (word >> 4 p) &
-// 0x000f000f put under the exponent of 128 (bfloat16) or 1024 (float16) is a pair q + 128 or q + 1024, and one packed
-// subtraction leaves q - z, exactly. float32 rows are the exact sum of three bfloat16 parts, one instruction each. The products
-// of a group are summed by the tensor core (at most eight steps of 16, the small parts first), then scaled and added in fp32.
-
-// For bfloat16 rows even that subtraction is left out: the instruction gets 128 + q, and (128 + z) times the group's sum of x -
-// one more pair of instructions with an operand of ones, shared by all output channels - is subtracted from the group's sum in
-// fp32. What that costs is the magnitude of the sums, about 30 times the result's: 5 of 24 bits, where the result keeps 8.
+// 0x000f000f put under the exponent of 2^-4 (bfloat16) or 1024 (float16) is a pair (q + 128) / 2048 or q + 1024, and one packed
+// subtraction leaves (q - z) / 2048 or q - z, exactly. float32 rows are the exact sum of three bfloat16 parts, one instruction each.
+// The products of a group are summed by the tensor core (at most eight steps of 16, the small parts first), then scaled and added in
+// fp32; the bfloat16 form's 2048 is multiplied in at the end. It keeps the sum of a group, at most 128 x 15 times the largest
+// magnitude, in range whatever x: bfloat16 and float32 rows reach to the end of fp32's, and the scales bring the result back.
+// (Giving the tensor core q + 128 and taking (128 + z) times the group's sum of x off afterwards carries 30 times the result's
+// magnitude, and without bound more where an x of weight 0 is large, and turns infinities into NaN; it was 1.5% faster on one bf16
+// row and 7% slower on 16.)
 
 // What bounds it: unpacking - 148 instructions per block of 2048 weights, at 16 warps per SM - more than memory. One bf16 row, on
 // the device: 4096 -> 14336 11.1 us (2.7 TB/s), 8192 -> 8192 11.6 us, 4096 -> 4096 5.1 us, 512 -> 512 2.1 us; 16 fp16 rows 8192 ->
 // 8192 with zero points 16.6 us; one float32 row 4096 -> 14336 17.6 us.
 
 template <typename T> struct W4Math {  // bfloat16; float32 in bfloat16 parts
-  static constexpr bool OFFSET = sizeof(T) == 2;  // the codes stay 128 above their value
-  static constexpr unsigned int MAGIC = 0x43004300u, ONES = 0x3f803f80u;
-  static __device__ __forceinline__ unsigned int zero_pair(unsigned int z) { return (0x4300u + z) * 0x10001u; }
+  static constexpr float UNIT = 2048.0f;  // what the sums are to be multiplied by
+  static constexpr unsigned int MAGIC = 0x3d803d80u;  // 2^-4, twice: its last place is 1 / 2048
+  static __device__ __forceinline__ unsigned int zero_pair(unsigned int z) { return (0x3d80u + z) * 0x10001u; }
   static __device__ __forceinline__ unsigned int sub(unsigned int a, unsigned int b) {
-    if (OFFSET) return a;
     const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
     return *reinterpret_cast<const unsigned int *>(&r);
   }
@@ -129,8 +129,8 @@ template <typename T> struct W4Math {  // bfloat16; float32 in bfloat16 parts
   }
 };
 template <> struct W4Math<__half> {
-  static constexpr bool OFFSET = false;
-  static constexpr unsigned int MAGIC = 0x64006400u, ONES = 0x3c003c00u;
+  static constexpr float UNIT = 1.0f;
+  static constexpr unsigned int MAGIC = 0x64006400u;
   static __device__ __forceinline__ unsigned int zero_pair(unsigned int z) { return (0x6400u + z) * 0x10001u; }
   static __device__ __forceinline__ unsigned int sub(unsigned int a, unsigned int b) {
     const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
@@ -240,6 +240,7 @@ __device__ __forceinline__ void store_out(const W4Args &a, int og, int row0, int
   const int l = e & 31, k = (e >> 5) & 3, n = (e >> 7) % NB, r = (e >> 7) / NB;
   const int o = (og * R + r) * kTileO + (k >> 1) * 8 + (l >> 2), row = row0 + n * 8 + (l & 3) * 2 + (k & 1);
   if (o < a.c_out && row < a.rows) {
+    v = __fmul_rn(v, W4Math<T>::UNIT);
     if (a.b) v = __fadd_rn(v, Elem<T>::to_f32(__ldg(static_cast<const T *>(a.b) + o)));
     static_cast<T *>(a.y)[(long long)row * a.ld_y + o] = Elem<T>::from_f32(v);
   }
@@ -309,7 +310,6 @@ __global__ void __launch_bounds__(256, 2) w4_affine_kernel(const W4Args a) {
     x0[n] = static_cast<const T *>(a.x) + (long long)(row < a.rows ? row : 0) * a.ld_x + it0 * kTileI + lc * 8;
   }
   const unsigned int magic = opaque_constant(M::MAGIC);
-  const unsigned int ones[4] = {M::ONES, M::ONES, M::ONES, M::ONES};
   const int i_left0 = a.c_in - it0 * kTileI - lc * 8;  // input channels from this lane's first one on
   int slot = 0, buf = 0;
   unsigned int ph = 0;
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(256, 2) w4_affine_kernel(const W4Args a) {
         ok = pw_wait(&bar[slot], ph);
         if (!ok) break;
       }
-      float part[R][NB][4], xsum[NB][4];
+      float part[R][NB][4];
       uint4 lo4[R], hi4[R];
       unsigned int z0[R], z1[R];
 #pragma unroll
@@ -361,11 +361,6 @@ __global__ void __launch_bounds__(256, 2) w4_affine_kernel(const W4Args a) {
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           const XFrag<T> x(raw[j][n]);
-          if (M::OFFSET) {  // every row of xsum is the group's sum of x
-            if (j % PER == 0) xsum[n][0] = xsum[n][1] = xsum[n][2] = xsum[n][3] = 0.0f;
-            M::mma(xsum[n], ones, x.w[0][0], x.w[0][1]);
-            M::mma(xsum[n], ones, x.w[0][2], x.w[0][3]);
-          }
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             const unsigned char *p = blk + r * (STEP * BLOCK);
@@ -391,11 +386,7 @@ __global__ void __launch_bounds__(256, 2) w4_affine_kernel(const W4Args a) {
               const T *sc = reinterpret_cast<const T *>(p + kTileBytes) + g * kTileO + lr;
               const float s0 = Elem<T>::to_f32(sc[0]), s1 = Elem<T>::to_f32(sc[8]);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                float v = part[r][n][k];
-                if (M::OFFSET) v = __fmaf_rn(xsum[n][k & 1], -__uint_as_float((k < 2 ? z0[r] : z1[r]) << 16), v);
-                acc[r][n][k] = __fmaf_rn(v, k < 2 ? s0 : s1, acc[r][n][k]);
-              }
+              for (int k = 0; k < 4; ++k) acc[r][n][k] = __fmaf_rn(part[r][n][k], k < 2 ? s0 : s1, acc[r][n][k]);
             }
           }
         }

@@ -46,3 +46,90 @@ def test_sixteen_bit_weight_gradients_have_no_bias(cuda_device, dt, rows, accum)
     # the roundings are spread evenly over +-half a step: their mean over n values is off by half / sqrt(3 n), times six
     assert err.mean().abs() <= drift + 6 * half / (3 * err.numel()) ** 0.5
     ops.check_device_flag()
+
+
+# ---- 4-bit weights -------------------------------------------------------------------------------
+
+
+def w4_layer(n, k, group, dtype, zero_points, device, seed):
+    g = gen(seed)
+    groups = (k + group - 1) // group
+    codes = torch.randint(0, 16, (n, k), generator=g).to(torch.uint8)
+    zeros = torch.randint(0, 16, (n, groups), generator=g).to(torch.uint8) if zero_points else None
+    scales = (torch.rand(n, groups, generator=g) * 0.004 + 0.002).to(dtype)
+    b = torch.randn(n, generator=g).to(dtype)
+    return codes, scales, zeros, b
+
+
+def packed(codes, scales, zeros, group, device):
+    return ops.pack_w4(codes.to(device), scales.to(device), None if zeros is None else zeros.to(device), group=group)
+
+
+def w4_bound(x, w, b, k, dtype):
+    """(64-bit result, limit): exact products, k of them and one bias added in fp32 (whatever the order, an adder that truncates
+    included), one rounding of the result. A weight of 0 takes no part, however large its x."""
+    want = x.double() @ w.T + b.double()
+    size = x.double().abs() @ w.abs().T + b.double().abs()
+    return want, (k + 8) * 2.0 ** -23 * size + want.abs() * fb.half_step(dtype) * 1.02
+
+
+@pytest.mark.parametrize("zero_points", [False, True], ids=["mid", "zeros"])
+@pytest.mark.parametrize("rows,k,n,group", [(3, 256, 48, 128), (11, 1000, 130, 64), (2, 520, 700, 32), (1, 4096, 4800, 128)])
+@pytest.mark.parametrize("dt", TYPES)
+def test_w4_values_that_are_not_finite_or_huge(cuda_device, dt, rows, k, n, group, zero_points):
+    """An infinity gives infinities of the weights' signs and NaN where the weight is 0; the largest number of the type gives numbers."""
+    dtype = fb.TYPES[dt]
+    top = torch.finfo(dtype).max
+    codes, scales, zeros, b = w4_layer(n, k, group, dtype, zero_points, cuda_device, k + n)
+    w4 = packed(codes, scales, zeros, group, cuda_device)
+    w = fb.w4_weight(codes, scales, zeros, group)
+    for case in (("inf", "-inf"), ("inf", "inf", "nan"), (top,), (top, -top, top), (top / 128, 1.0)):
+        x = torch.randn(rows, k, generator=gen(len(case))).to(dtype)
+        for i, v in enumerate(case):
+            x[-1, (37 * i + 5) % k] = float(v)
+        got = ops.affine_w4(x.to(cuda_device), w4, b.to(cuda_device)).cpu().double()
+        want, lim = w4_bound(x, w, b, k, dtype)
+        fin = want.isfinite()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf() & ~fin, want.isinf())
+        assert torch.equal(got[want.isinf()], want[want.isinf()])
+        assert ((got - want).abs() <= lim)[fin].all()
+        assert fin[:-1].all() and (not isinstance(case[0], float) or fin.all())
+    ops.check_device_flag()
+
+
+@pytest.mark.parametrize("outlier", [1e2, 1e4, 6e4])
+@pytest.mark.parametrize("rows,k,n,group", [(1, 1024, 160, 128), (16, 640, 64, 32), (2, 512, 4800, 64)])
+@pytest.mark.parametrize("dt", TYPES)
+def test_w4_outliers_of_unused_channels(cuda_device, dt, rows, k, n, group, outlier):
+    """One channel of every group is far larger than the others and has weight 0: it does not show in the result."""
+    dtype = fb.TYPES[dt]
+    codes, scales, zeros, b = w4_layer(n, k, group, dtype, True, cuda_device, 3)
+    idle = torch.arange(0, k, group) + 17 % group
+    codes[:, idle] = zeros
+    x = torch.randn(rows, k, generator=gen(5)).to(dtype)
+    x[:, idle] = outlier
+    want, lim = w4_bound(x, fb.w4_weight(codes, scales, zeros, group), b, k, dtype)
+    got = ops.affine_w4(x.to(cuda_device), packed(codes, scales, zeros, group, cuda_device), b.to(cuda_device)).cpu().double()
+    assert ((got - want).abs() <= lim).all()
+    # rows with a large common part, which cancels where a group's weights do (float16: so large that the results stay in range)
+    x = (outlier / (64 if dtype == torch.float16 else 1) + torch.randn(rows, k, generator=gen(6))).to(dtype)
+    want, lim = w4_bound(x, fb.w4_weight(codes, scales, zeros, group), b, k, dtype)
+    got = ops.affine_w4(x.to(cuda_device), packed(codes, scales, zeros, group, cuda_device), b.to(cuda_device)).cpu().double()
+    assert ((got - want).abs() <= lim).all()
+
+
+@pytest.mark.parametrize("rows", [1, 12])
+@pytest.mark.parametrize("dt", TYPES)
+def test_w4_weights_of_zero_give_the_bias(cuda_device, dt, rows):
+    dtype, n, k, group = fb.TYPES[dt], 4800, 1100, 64
+    codes, scales, zeros, b = w4_layer(n, k, group, dtype, True, cuda_device, 8)
+    codes = zeros.repeat_interleave(group, 1)[:, :k].contiguous()
+    x = (100 + torch.randn(rows, k, generator=gen(7))).to(dtype)
+    got = ops.affine_w4(x.to(cuda_device), packed(codes, scales, zeros, group, cuda_device), b.to(cuda_device))
+    assert torch.equal(got.cpu(), b.expand(rows, n))
+    # groups whose scale is not finite stand for NaN
+    scales[5, 2], scales[7, 0] = float("nan"), float("inf")
+    got = ops.affine_w4(x.to(cuda_device), packed(codes, scales, zeros, group, cuda_device), b.to(cuda_device)).cpu()
+    bad = torch.zeros(rows, n, dtype=torch.bool)
+    bad[:, 5] = bad[:, 7] = True
+    assert torch.equal(got.isnan(), bad) and torch.equal(got[~bad], b.expand(rows, n)[~bad])
