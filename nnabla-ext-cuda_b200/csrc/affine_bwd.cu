@@ -169,7 +169,7 @@ static_assert(kStageBytes % 1024 == 0 && kStages * (kStageBytes + kExpBytes) + 1
 // pw_wait for a warp of a CTA that may be giving up: the flag is looked at only when the barrier is not ready.
 __device__ __forceinline__ bool dw_wait(unsigned long long *bar, unsigned int parity, volatile int *abort_v) {
   if (__all_sync(0xffffffffu, pw_try_wait(bar, parity))) return true;
-  return pw_wait(bar, parity) && !*abort_v;
+  return pw_wait(bar, parity) && !pw_giving_up(abort_v);
 }
 
 // The pointer, in a way the compiler cannot compute ahead of: all columns' addresses at once would not fit the registers.

@@ -48,6 +48,8 @@ __device__ __forceinline__ bool pw_wait(unsigned long long *bar, unsigned int pa
   }
   return ok;
 }
+// Whether a warp of the CTA is giving up (*abort_v): one answer for the whole warp, whose lanes may read the word at different times.
+__device__ __forceinline__ bool pw_giving_up(volatile int *abort_v) { return __any_sync(0xffffffffu, *abort_v != 0); }
 // (a & mask) | set as one instruction. A logic instruction takes one immediate: with both constants known the compiler needs two,
 // so `set` has to come from a value it cannot see through (opaque_constant).
 __device__ __forceinline__ unsigned int and_or(unsigned int a, unsigned int mask, unsigned int set) {

@@ -386,7 +386,7 @@ pw_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ C
       int s = 0;
       unsigned int ph = 0;
       auto store = [&](const float4(&v)[4]) -> bool {
-        if (!pw_wait(&empty[s], ph ^ 1u) || *abort_v) return false;
+        if (!pw_wait(&empty[s], ph ^ 1u) || pw_giving_up(abort_v)) return false;
         unsigned char *xh = sm + (size_t)s * a.stage_bytes + sw4;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -474,7 +474,7 @@ pw_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ C
       int s = 0;
       unsigned int ph = 0;
       auto store = [&](const float(&v)[16]) -> bool {
-        if (!pw_wait(&empty[s], ph ^ 1u) || *abort_v) return false;
+        if (!pw_wait(&empty[s], ph ^ 1u) || pw_giving_up(abort_v)) return false;
         // row k = 16 kh + j of the chunk: k mod 4 = j mod 4, so four base addresses serve all rows
         unsigned char *xh = sm + (size_t)s * a.stage_bytes + sw_base + kh * 2048;
         unsigned char *const rb[4] = {xh + ((unit ^ 0u) << 5), xh + ((unit ^ 1u) << 5), xh + ((unit ^ 2u) << 5),
@@ -520,7 +520,7 @@ pw_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ C
       bool ok = true;
       for (int t = blockIdx.x; ok && t < a.total_tiles; t += gridDim.x) {
         for (int kc = 0; kc < a.kchunks; ++kc) {
-          ok = pw_wait(&full[s], ph) && !*abort_v;
+          ok = pw_wait(&full[s], ph) && !pw_giving_up(abort_v);
           if (!ok) break;
           uint4 *xh = reinterpret_cast<uint4 *>(sm + (size_t)s * a.stage_bytes);
           uint4 *xl = reinterpret_cast<uint4 *>(sm + (size_t)s * a.stage_bytes + off_xlo);
@@ -593,7 +593,7 @@ pw_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ C
         p = (r - (int)n * a.pos_tiles) * kPwPosTile + quarter * 32 + lane;
         p_ok = p < a.HW;
       }
-      if (!pw_wait(&acc_full[b], aph) || *abort_v) {
+      if (!pw_wait(&acc_full[b], aph) || pw_giving_up(abort_v)) {
         if (lane == 0 && !*abort_v) { atomicExch(a.flag, 1); *abort_v = 1; }
         break;
       }
