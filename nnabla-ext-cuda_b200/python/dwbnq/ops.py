@@ -535,6 +535,8 @@ def affine_weight_backward(ck_x, dy, dw=None, db=None, need=(True, True), accum=
     code = _few_bits_code(dy.dtype)
     if ck_x.shape[:-1] != tuple(dy.shape[:-1]):
         raise ValueError("dy %s has other rows than the checkpoint %s" % (tuple(dy.shape), ck_x.shape))
+    if ws is not None and not ws.is_contiguous():
+        raise ValueError("ws must be contiguous")
     if any(a and n and t is None for a, n, t in zip(accum, need, (dw, db))):
         raise ValueError("accumulating needs the tensor to accumulate onto")
     if dtype is None:
