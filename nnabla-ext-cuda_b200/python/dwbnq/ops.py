@@ -564,12 +564,26 @@ def affine_weight_backward(ck_x, dy, dw=None, db=None, need=(True, True), accum=
 
 
 class W4Weight:
-    """4-bit weights [c_out, c_in] laid out for affine_w4 (``packed``), with the type of the layer's tensors."""
+    """4-bit weights [c_out, c_in] laid out for affine_w4 (``packed``: the bytes that pack_w4 made), with the type of the layer's
+    tensors. ``packed`` may be None until it is set."""
 
     def __init__(self, packed, c_out, c_in, group, dtype, has_zeros):
-        self.packed, self.c_out, self.c_in, self.group, self.dtype, self.has_zeros = packed, c_out, c_in, group, dtype, has_zeros
+        self.c_out, self.c_in, self.group, self.dtype, self.has_zeros = c_out, c_in, group, dtype, has_zeros
         self._desc = L.W4Desc(dtype=_few_bits_code(dtype), group=group, c_in=c_in, c_out=c_out, has_zeros=int(has_zeros))
         self._ref = ctypes.byref(self._desc)
+        self.packed = packed
+
+    @property
+    def packed(self):
+        return self._packed
+
+    @packed.setter
+    def packed(self, t):
+        if t is not None:
+            need = int(L.lib().dwbnq_w4_packed_bytes(self._ref))
+            if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() < need:
+                raise ValueError("packed must be contiguous uint8 of %d bytes for this layer" % need)
+        self._packed = t
 
     def desc(self):
         """The layer's dwbnq_w4_desc, by reference."""
@@ -620,8 +634,11 @@ def affine_w4(x, w4, b=None, out=None):
     y = _like(out, "out", x.shape[:-1] + (w4.c_out,), x.dtype, x.device, x)
     if b is not None and not _like(b, "b", (w4.c_out,), x.dtype, x.device).is_contiguous():
         raise ValueError("b must be contiguous")
-    dev = _one_device(x, w4.packed, b, y)
-    _launch("dwbnq_w4_affine_fwd", dev, w4.desc(), rows, ldx, x.data_ptr(), w4.packed.data_ptr(), _addr(b),
+    packed = w4.packed
+    if packed is None:
+        raise ValueError("the layer has no packed weights yet")
+    dev = _one_device(x, packed, b, y)
+    _launch("dwbnq_w4_affine_fwd", dev, w4.desc(), rows, ldx, x.data_ptr(), packed.data_ptr(), _addr(b),
             _rows_view(y, "out")[2], y.data_ptr())
     return y
 

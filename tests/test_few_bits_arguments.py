@@ -20,3 +20,25 @@ def test_a_workspace_is_memory_of_its_size():
                torch.zeros(1 << 12, 1 << 12, dtype=torch.uint8)[:, ::2], torch.zeros(64, 1 << 17).T):
         with pytest.raises(ValueError, match="ws must be contiguous"):
             ops.affine_weight_backward(checkpoint(), dy, ws=ws)
+
+
+def test_packed_weights_are_as_large_as_their_layer():
+    """Packed weights kept by the caller (from a file, of another layer or group size) are checked where they are given."""
+    need = 2048 + 256  # 8 channels of 240 in groups of 128: two blocks of 1 KiB, 2 x 16 scales of 2 bytes each
+    new = lambda packed, **kw: ops.W4Weight(packed, *(kw.get(k, v) for k, v in (("c_out", 8), ("c_in", 240), ("group", 128))),  # noqa: E731
+                                            torch.bfloat16, False)
+    assert new(torch.zeros(need, dtype=torch.uint8)).packed.numel() == need
+    assert new(torch.zeros(need + 5, dtype=torch.uint8)).packed is not None
+    for bad in (torch.zeros(need - 256, dtype=torch.uint8), torch.zeros(need), torch.zeros(1, dtype=torch.uint8).expand(need),
+                torch.zeros(2 * need, dtype=torch.uint8)[::2], torch.zeros(need, dtype=torch.int8)):
+        with pytest.raises(ValueError, match="packed"):
+            new(bad)
+        w4 = new(torch.zeros(need, dtype=torch.uint8))
+        with pytest.raises(ValueError, match="packed"):
+            w4.packed = bad
+    for other in (dict(c_in=257), dict(c_out=17), dict(c_in=512, group=32)):
+        with pytest.raises(ValueError, match="packed"):
+            new(torch.zeros(need, dtype=torch.uint8), **other)
+    w4 = new(None)
+    with pytest.raises(ValueError, match="packed"):
+        ops.affine_w4(torch.zeros(1, 240, dtype=torch.bfloat16), w4)
