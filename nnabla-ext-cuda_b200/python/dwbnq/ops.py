@@ -590,16 +590,23 @@ class W4Weight:
         return self._ref
 
 
+def _w4_groups(c_in, group):
+    if group not in (32, 64, 128):
+        raise L.DwbnqError(L.ERR_UNSUPPORTED, "group of %s input channels: 32, 64 and 128 are supported" % (group,))
+    return (c_in + group - 1) // group
+
+
 def quantize_w4(w, group=128):
     """Round-to-nearest 4-bit weights of w [c_out, c_in]: (codes uint8 [c_out, c_in] in 0..15, scales [c_out, groups]);
     the weight is (code - 8) * scale. Lay them out with pack_w4."""
     if w.dim() != 2:
         raise ValueError("w must be [c_out, c_in]")
     code = _few_bits_code(w.dtype)
+    groups = _w4_groups(int(w.shape[1]), group)
     dev = _one_device(w)
     c_out, c_in, ld = _rows_view(w, "w")
     codes = torch.empty((c_out, c_in), dtype=torch.uint8, device=dev)
-    scales = torch.empty((c_out, (c_in + group - 1) // group), dtype=w.dtype, device=dev)
+    scales = torch.empty((c_out, groups), dtype=w.dtype, device=dev)
     _launch("dwbnq_w4_quantize", dev, code, c_out, c_in, group, ld, _addr(w), _addr(codes), _addr(scales))
     return codes, scales
 
@@ -610,7 +617,7 @@ def pack_w4(codes, scales, zeros=None, group=128):
     if codes.dim() != 2 or codes.dtype != torch.uint8:
         raise ValueError("codes must be uint8 [c_out, c_in]")
     c_out, c_in = (int(s) for s in codes.shape)
-    groups = (c_in + group - 1) // group
+    groups = _w4_groups(c_in, group)
     dev = _one_device(codes, scales, zeros)
     _like(scales, "scales", (c_out, groups), scales.dtype, dev)
     if zeros is not None:

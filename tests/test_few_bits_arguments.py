@@ -42,3 +42,13 @@ def test_packed_weights_are_as_large_as_their_layer():
     w4 = new(None)
     with pytest.raises(ValueError, match="packed"):
         ops.affine_w4(torch.zeros(1, 240, dtype=torch.bfloat16), w4)
+
+
+@pytest.mark.parametrize("group", [0, -32, 16, 48, 256])
+def test_group_sizes_are_refused_alike(group):
+    """A group size that does not exist is the library's refusal, whatever the number."""
+    codes, scales = torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 4)
+    for call in (lambda: ops.quantize_w4(torch.zeros(4, 64), group=group), lambda: ops.pack_w4(codes, scales, group=group)):
+        with pytest.raises(L.DwbnqError) as e:
+            call()
+        assert e.value.status == L.ERR_UNSUPPORTED
