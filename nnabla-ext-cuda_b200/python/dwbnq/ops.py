@@ -455,6 +455,8 @@ def _ck_out(ck, name, shape, dtype, like):
 def checkpoint_code8(x, out=None):
     """The 8-bit checkpoint of x [..., channels] (groups of 32 channels share a power-of-two step)."""
     code = _few_bits_code(x.dtype)
+    if x.dim() < 1:
+        raise ValueError("x must have at least one axis")
     ck = _ck_out(out, "out", x.shape, x.dtype, x)
     dev = _one_device(x, ck.codes, ck.exponents)
     rows, cols, ld = _rows_view(x, "x")

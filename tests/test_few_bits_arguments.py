@@ -52,3 +52,10 @@ def test_group_sizes_are_refused_alike(group):
         with pytest.raises(L.DwbnqError) as e:
             call()
         assert e.value.status == L.ERR_UNSUPPORTED
+
+
+def test_tensors_without_an_axis_are_refused():
+    one = torch.zeros(())
+    for call in (lambda: ops.checkpoint_code8(one), lambda: ops.glu(one, one), lambda: ops.affine_weight_backward(checkpoint(), one)):
+        with pytest.raises(ValueError):
+            call()
