@@ -133,3 +133,51 @@ def test_w4_weights_of_zero_give_the_bias(cuda_device, dt, rows):
     bad = torch.zeros(rows, n, dtype=torch.bool)
     bad[:, 5] = bad[:, 7] = True
     assert torch.equal(got.isnan(), bad) and torch.equal(got[~bad], b.expand(rows, n)[~bad])
+
+
+# ---- gated unit ----------------------------------------------------------------------------------
+
+MAGNITUDES = [1e-30, 1e-8, 2.0 ** -14, 1e-3, 0.1, 0.5, 0.75, 1.0, 1.2785, 1.5, 2.0, 2.75, 3.0, 4.0, 5.5, 7.0, 9.0, 11.0, 13.0, 13.25, 15.0, 16.0,
+              17.5, 20.0, 40.0, 64.0, 87.0, 88.0, 89.0, 100.0, 104.0, 500.0, 6e4, 1e10, 1e19, 1e30, 3e38]
+
+
+def act_near(got, want, size, g, scale, dtype):
+    """One rounding to the type; the evaluation in fp32, 24 half-steps of the terms' size and the rounding of an exponential's argument
+    (3 |g|; 4 g^2 where the exponential is of g^2, whose results vanish beyond 15); and 0 for what fp32 holds below 2^-126."""
+    unit = 24 + 3 * g.abs() + 4 * torch.clamp(g * g, max=225.0)
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    lim = want.abs() * fb.half_step(dtype) * 1.02 + tiny + unit * 2.0 ** -24 * size + 2.0 ** -125 * (g.abs() + 1) * scale
+    bad = ~((got.double().cpu() - want).abs() <= lim)
+    assert not bad.any(), (g[bad][:4], got.cpu()[bad][:4], want[bad][:4], lim[bad][:4])
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("dt", TYPES)
+def test_glu_over_the_whole_range(cuda_device, dt, act):
+    """Both signs of every size that the type holds, a group of 32 each, forward and backward."""
+    dtype = fb.TYPES[dt]
+    top = torch.finfo(dtype).max
+    m = torch.tensor([v for v in MAGNITUDES if v <= top and v >= torch.finfo(dtype).smallest_normal], dtype=torch.float64)
+    steps = torch.tensor([1.0, 0.99, 0.9, 0.75, 0.6, 0.51, 0.3, 0.1] * 2, dtype=torch.float64)
+    gate = (m[:, None] * torch.cat([steps, -steps])).to(dtype)
+    up = torch.full_like(gate, 0.5)
+    up[:, ::3] = -1.0
+    dy = torch.full_like(gate, 2.0)
+    y, cg, cu = ops.glu(gate.to(cuda_device), up.to(cuda_device), act=act, checkpoint=True)
+    g, u = gate.double(), up.double()
+    a, _, _ = fb.act(act, g)
+    act_near(y, a * u, (a * u).abs(), g, u.abs(), dtype)
+    dg, du = ops.glu_backward(cg, cu, dy.to(cuda_device), act=act)
+    gv, uv = fb.ckpt8(gate)[2], fb.ckpt8(up)[2]
+    a, d, size = fb.act(act, gv)
+    act_near(dg, 2 * uv * d, (2 * uv).abs() * size, gv, (2 * uv).abs(), dtype)
+    inside = (2 * a).abs() < top * 0.999
+    act_near(du.cpu()[inside], (2 * a)[inside], (2 * a).abs()[inside], gv[inside], torch.full_like(gv, 2.0)[inside], dtype)
+    assert torch.equal(du.cpu().double()[~inside], (2 * a)[~inside].to(dtype).double())
+    # what is not finite
+    g = torch.tensor([[float("inf"), float("-inf"), float("nan"), 0.0, -0.0, 1.0]]).to(dtype)
+    y = ops.glu(g.to(cuda_device), torch.ones_like(g).to(cuda_device), act=act).cpu()
+    want = fb.act(act, g.double())[0].to(dtype)
+    if act == "relu":
+        want = torch.tensor([[float("inf"), 0.0, float("nan"), 0.0, 0.0, 1.0]]).to(dtype)
+    assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y.nan_to_num(nan=7.0, posinf=9.0)[:, :5], want.nan_to_num(nan=7.0, posinf=9.0)[:, :5])
