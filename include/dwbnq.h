@@ -456,8 +456,10 @@ size_t dwbnq_affine_bwd_workspace_bytes(const dwbnq_affine_desc *desc);
 /* Weight and bias gradients with the input read from its checkpoint (codes and exps of x [rows,
  * c_in]): dw[o][i] (+)= sum over rows of dy[r][o] * x[r][i], dw [c_out, c_in] contiguous;
  * db[o] (+)= sum over rows of dy[r][o]. dw and db may each be NULL. accum_mask bit 1 / 2:
- * accumulate onto dw / db (as in dwbnq_dwconv_bwd). Products are exact, sums are kept in fp32, their
- * order is fixed: the same call gives the same bits. */
+ * accumulate onto dw / db (as in dwbnq_dwconv_bwd). Products are exact (of a float32 dy, what lies
+ * below 2^-133 is dropped), sums are kept in fp32, in runs of at most 512 tokens (4096 for the lower
+ * digits of a float16 or float32 dy) that the tensor cores add up; their order is fixed: the same call
+ * gives the same bits. */
 int dwbnq_affine_bwd_ckpt8(const dwbnq_affine_desc *desc, const void *codes, const void *exps, const void *dy, void *dw,
                            void *db, int accum_mask, void *workspace, int device, void *stream);
 

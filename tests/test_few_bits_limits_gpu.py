@@ -181,3 +181,66 @@ def test_glu_over_the_whole_range(cuda_device, dt, act):
     if act == "relu":
         want = torch.tensor([[float("inf"), 0.0, float("nan"), 0.0, 0.0, 1.0]]).to(dtype)
     assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y.nan_to_num(nan=7.0, posinf=9.0)[:, :5], want.nan_to_num(nan=7.0, posinf=9.0)[:, :5])
+
+
+# ---- gradients near the end of the range -------------------------------------------------------------
+
+
+@pytest.mark.parametrize("exponent", [-100, -109, -113, -120, -127])
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_weight_gradient_of_tiny_dy(cuda_device, dt, exponent):
+    """A dy down to the last numbers below the normal range, times an x that brings the result back."""
+    dtype, rows, c_in, c_out = fb.TYPES[dt], 200, 96, 40
+    x = torch.randn(rows, c_in, generator=gen(1)) * 2.0 ** 90
+    dy = (torch.randn(rows, c_out, generator=gen(2)).double() * 2.0 ** exponent).to(dtype)
+    ck = ops.checkpoint_code8(x.to(cuda_device))
+    xv = fb.ckpt8(x)[2]
+    want, size = dy.double().T @ xv, dy.double().abs().T @ xv.abs()
+    dw, db = ops.affine_weight_backward(ck, dy.to(cuda_device), dtype=torch.float32)
+    # float32: the last of the three parts ends at bfloat16's last number, 2^-133
+    lost = 2.0 ** -133 * xv.abs().sum(0) if dt == "f32" else torch.zeros(c_in, dtype=torch.float64)
+    assert ((dw.cpu().double() - want).abs() <= (rows + 8) * 2.0 ** -23 * size + lost).all()
+    wantb = dy.double().sum(0)
+    assert ((db.cpu().double() - wantb).abs() <= (rows + 8) * 2.0 ** -24 * dy.double().abs().sum(0) + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_checkpoints_and_weights_near_zero(cuda_device, dt):
+    """4-bit weights and rows whose products lie below the normal range of the type, brought back by the other factor."""
+    dtype, rows, k, n, group = fb.TYPES[dt], 5, 256, 96, 64
+    small, large = (2.0 ** -14, 1.0) if dt == "f16" else (2.0 ** -110, 2.0 ** 100)
+    codes, scales, zeros, _ = w4_layer(n, k, group, torch.float32, True, cuda_device, 4)
+    for xs, ss in ((small, large), (large, small)):
+        x = (torch.randn(rows, k, generator=gen(3)).double() * xs).to(dtype)
+        s = (scales.double() * ss).to(dtype)
+        w = fb.w4_weight(codes, s, zeros, group)
+        want, lim = w4_bound(x, w, torch.zeros(n), k, dtype)
+        lim = lim + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+        if dt == "f32":  # the parts of a row end at 2^-133
+            lim = lim + 2.0 ** -133 * w.abs().sum(1)
+        got = ops.affine_w4(x.to(cuda_device), packed(codes, s, zeros, group, cuda_device)).cpu().double()
+        assert ((got - want).abs() <= lim).all()
+
+
+@pytest.mark.parametrize("rows,c_in,c_out", [(1, 4500, 5000), (70, 4096, 6000), (129, 256, 20000), (600, 1024, 1100)])
+@pytest.mark.parametrize("dt", TYPES)
+def test_weight_gradient_units_of_every_length(cuda_device, dt, rows, c_in, c_out):
+    """More tiles than SMs with one chunk of tokens each, two or a few; the exponents on and off a word boundary, accumulated too."""
+    dtype = fb.TYPES[dt]
+    g = torch.Generator(device=cuda_device).manual_seed(rows)
+    # whole numbers: every sum is exact
+    x = torch.randint(-127, 128, (rows, c_in), generator=g, device=cuda_device).float()
+    x[:, ::32] = 127
+    dy = torch.randint(-4, 5, (rows, c_out), generator=g, device=cuda_device).to(dtype)
+    want = (dy.double().T @ x.double()).float()
+    ck = ops.checkpoint_code8(x)
+    buf = torch.zeros(ck.exponents.numel() + 1, dtype=torch.uint8, device=cuda_device)
+    buf[1:] = ck.exponents.flatten()
+    odd = ops.Code8Checkpoint(ck.codes, buf[1:].view(ck.exponents.shape), ck.shape, ck.dtype)
+    for c in (ck, odd):
+        dw, _ = ops.affine_weight_backward(c, dy, need=(True, False), dtype=torch.float32)
+        assert torch.equal(dw, want)
+        assert torch.equal(ops.affine_weight_backward(c, dy, need=(True, False))[0], want.to(dtype))
+    acc, _ = ops.affine_weight_backward(odd, dy, dw=torch.ones_like(want), need=(True, False), accum=(True, False))
+    assert torch.equal(acc, want + 1)
+    ops.check_device_flag()
