@@ -102,9 +102,11 @@ __global__ void __launch_bounds__(256)
 // magnitude, and without bound more where an x of weight 0 is large, and turns infinities into NaN; it was 1.5% faster on one bf16
 // row and 7% slower on 16.)
 
-// What bounds it: unpacking - 148 instructions per block of 2048 weights, at 16 warps per SM - more than memory. One bf16 row, on
-// the device: 4096 -> 14336 11.1 us (2.7 TB/s), 8192 -> 8192 11.6 us, 4096 -> 4096 5.1 us, 512 -> 512 2.1 us; 16 fp16 rows 8192 ->
-// 8192 with zero points 16.6 us; one float32 row 4096 -> 14336 17.6 us.
+// What bounds it: nothing is saturated. For one bf16 row 4096 -> 14336 the 172 instructions per block of 2048 weights fill 4.4 of 11 us
+// of issue slots, DRAM runs at a quarter of its rate and the tensor cores at a sixth: there are 16 warps per SM at most, each waits
+// for its own copy, and the tiles of 16 x R channels do not come out even (224 CTAs here: half the SMs have one, half two). On the
+// device: one bf16 row 4096 -> 14336 11.4 us (2.65 TB/s), 8192 -> 8192 11.9 us, 4096 -> 4096 5.1 us, 512 -> 512 2.1 us; one float16 row
+// 4096 -> 14336 10.4 us, one float32 row 17.6 us; 16 rows: bf16 4096 -> 14336 17.4 us, fp16 8192 -> 8192 with zero points 16.6 us.
 
 template <typename T> struct W4Math {  // bfloat16; float32 in bfloat16 parts
   static constexpr float UNIT = 2048.0f;  // what the sums are to be multiplied by
@@ -495,10 +497,13 @@ int affine_launch(W4Args a, int warps, int cluster, int ctas, cudaStream_t strea
 }
 // Output tiles per warp: a warp's rows of x, its waits and its loop cost the same for one tile and for four, but fewer warps are at
 // work. With enough weights for every SM (27 blocks) a warp takes four tiles where that leaves a group for every SM, else two where
-// that leaves one for every second SM (one bf16 row, us with 4 / 2 tiles: 4096 -> 14336 11.2 / 13.0, 4096 -> 4096 7.6 / 5.1, 14336
-// -> 4096 16.5 / 11.3); with fewer weights one (512 -> 512: 2.1 against 3.1 with four). Rows 9 to 16 double the accumulators: two at
-// most (4096 -> 14336, 16 rows: 19.1 against 25.0). Two CTAs fit an SM; while there are fewer, a cluster of CTAs divides the
-// input channels of each group, and where there are more they walk over the groups in equal rounds.
+// that leaves one for every second SM (one bf16 row, us with 4 / 2 / 1 tiles: 4096 -> 14336 11.4 / 12.3 / 14.1, 8192 -> 8192 12.0 /
+// 11.9 / 13.4, 4096 -> 4096 5.5 / 5.1 / 5.2, 14336 -> 4096 15.8 / 11.5 / 11.8; float32 4096 -> 14336 17.6 / 20.4 / 27.9); with fewer weights
+// one (512 -> 512: 3.0 / 2.4 / 2.1). Rows 9 to 16 double the accumulators: two at most (4096 -> 14336, 16 bf16 rows: 23.2 / 17.4 / 21.6).
+// Two CTAs fit an SM; while there are fewer, a cluster of CTAs divides the input channels of each group, and where there are more
+// they walk over the groups in equal rounds. The plan does not look at what a type and group size need: float32 in groups of 32 with
+// zero points has shared memory for one CTA where a warp takes four tiles, which then run one after the other (4096 -> 14336 25.3 us,
+// 21.7 with two tiles), and the four-tile float32 and 16-row float32 forms spill some registers.
 template <typename T, int G, bool ZEROS>
 int affine_g(const W4Args &a, cudaStream_t stream) {
   const bool many = (long long)a.o_tiles * a.i_tiles >= 27LL * kPlanSms;

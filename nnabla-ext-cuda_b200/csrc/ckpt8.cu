@@ -1,5 +1,6 @@
 // 8-bit activation checkpoints: writing one from a tensor, and reading it back. Both are bound by memory (3.03 bytes per 16-bit
-// value each way, a dozen instructions): a lane has eight values, so that its access is 16 bytes and four lanes share a group; two
+// value each way, a dozen instructions), the restoring of 16-bit values also by its grid - eight CTAs per SM are launched, five fit
+// with its registers, so that the last ones run by themselves: a lane has eight values, so that its access is 16 bytes and four lanes share a group; two
 // such accesses in flight per thread when writing, four of the 8-byte ones when reading. [16384, 8192] bf16: written in 83 us
 // (4.9 TB/s), restored in 97 us (4.2 TB/s; most of its bytes are stores); fp32 122 and 130 us (5.5 and 5.2 TB/s).
 #include "ckpt8.cuh"

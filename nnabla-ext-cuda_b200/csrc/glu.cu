@@ -5,7 +5,8 @@
 //   relu(g) = max(g, 0)                          relu'(g) = 1 for g > 0, else 0
 // dup = dy act(g), dgate = dy up act'(g), product = act(g) up, all in fp32, rounded once to the tensors' type.
 // Bound by memory (8.06 bytes per value forward with checkpoints, 8.06 backward, bf16), with the arithmetic close behind: about 40
-// instructions per value leave a third of the issue slots. One pass, eight values per lane. [8192, 11008] bf16: silu forward with
+// instructions per value leave a third of the issue slots; and by the grid of eight CTAs per SM, of which six (16-bit forward) and
+// five (16-bit backward) fit at a time. One pass, eight values per lane. [8192, 11008] bf16: silu forward with
 // checkpoints 141 us (5.1 TB/s), backward 166 us (4.4 TB/s); gelu 167 and 196 us; fp32 silu 226 us each way (5.6 TB/s).
 #include "ckpt8.cuh"
 #include "dwbnq_internal.h"
