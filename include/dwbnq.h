@@ -488,7 +488,8 @@ int dwbnq_w4_pack(const dwbnq_w4_desc *desc, const void *codes, const void *scal
 /* y = x w^T + b for a few rows (one token, or one token of each of a batch of sequences):
  * x [rows, c_in], y [rows, c_out] with row strides ld_x and ld_y, b [c_out] or NULL. The weights
  * are read once per 16 rows. Products x * (q - z) are exact and summed in fp32, a group's sum is then scaled. An
- * infinite or NaN x gives what the formula gives; a scale that is not finite makes its channel's results so. */
+ * infinite or NaN x gives what the formula gives; a scale that is not finite makes its channel's results so. Float32
+ * rows and results below 2^-110 keep fewer digits than above. */
 int dwbnq_w4_affine_fwd(const dwbnq_w4_desc *desc, int64_t rows, int64_t ld_x, const void *x, const void *packed,
                         const void *b, int64_t ld_y, void *y, int device, void *stream);
 

@@ -643,7 +643,7 @@ def affine_w4(x, w4, b=None, out=None):
     y = _like(out, "out", x.shape[:-1] + (w4.c_out,), x.dtype, x.device, x)
     if b is not None and not _like(b, "b", (w4.c_out,), x.dtype, x.device).is_contiguous():
         raise ValueError("b must be contiguous")
-    packed = w4.packed
+    packed = w4._packed
     if packed is None:
         raise ValueError("the layer has no packed weights yet")
     dev = _one_device(x, packed, b, y)
