@@ -244,3 +244,34 @@ def test_weight_gradient_units_of_every_length(cuda_device, dt, rows, c_in, c_ou
     acc, _ = ops.affine_weight_backward(odd, dy, dw=torch.ones_like(want), need=(True, False), accum=(True, False))
     assert torch.equal(acc, want + 1)
     ops.check_device_flag()
+
+
+FIRST_CALL = """
+import sys, torch
+sys.path[:0] = sys.argv[1:]
+from dwbnq import ops
+x, dy = torch.randn(300, 256, device="cuda").half(), torch.randn(300, 200, device="cuda").half()
+codes, scales = torch.randint(0, 16, (96, 256), device="cuda", dtype=torch.uint8), torch.rand(96, 2, device="cuda").half()
+def step():
+    y, cg, cu = ops.glu(x, x, checkpoint=True)
+    dg, du = ops.glu_backward(cg, cu, x)
+    dw, db = ops.affine_weight_backward(ops.checkpoint_code8(y), dy, dtype=torch.float32)
+    return dg, du, dw, db, ops.affine_w4(x[:5], ops.pack_w4(codes, scales))
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = step()
+x.copy_(torch.randn(300, 256, device="cuda"))
+g.replay()
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+ops.check_device_flag()
+print("same")
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured(cuda_device):
+    import os
+    import subprocess
+    import sys
+    paths = [os.path.dirname(os.path.dirname(os.path.abspath(ops.__file__)))]
+    out = subprocess.run([sys.executable, "-c", FIRST_CALL] + paths, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.strip() == "same", out.stderr[-2000:]
